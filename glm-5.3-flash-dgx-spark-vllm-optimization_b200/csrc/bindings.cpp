@@ -1048,6 +1048,7 @@ void rejection_sample(const Tensor& target_probs, const Tensor& draft_probs, con
 }  // namespace
 
 void register_exl3_codec(pybind11::module& m);   // exl3_codec.cpp (host codec)
+void register_fp4(pybind11::module& m);          // fp4_bind.cpp (4-bit floating-point operators)
 
 namespace {
 // (enabled, [(code, index, limit, count), ...]) of the bounds-checked build's records that saw an error
@@ -1075,6 +1076,7 @@ void bounds_reset() {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_exl3_codec(m);
+  register_fp4(m);
   m.doc() = "glm53 sm_100a kernels";
   m.def("gemv", &gemv, py::arg("x"), py::arg("w"), py::arg("scale"), py::arg("y"), py::arg("mode"), py::arg("limit"),
         py::arg("ks") = 0, py::arg("cl") = 0);

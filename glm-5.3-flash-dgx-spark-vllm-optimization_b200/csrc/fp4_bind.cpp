@@ -1,0 +1,296 @@
+// Python bindings of the 4-bit floating-point operators: argument checks, dispatch by row count, launches on the current
+// stream of the tensors' device.  Temporaries come from the caching allocator inside the call, so calls on different
+// streams, and captured graphs, never share one.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <string>
+
+#include "launchers.h"
+
+namespace {
+
+using at::Tensor;
+using OptT = c10::optional<Tensor>;
+
+constexpr int64_t kTileRows = 128, kTileK = 256, kTileBytes = 16384;
+constexpr int64_t kGemvRows = 16;      // rows of one small-M launch
+constexpr int64_t kGemmRows = 64;      // rows from which exact activations go through the bf16 tcgen05 GEMM
+
+void ok(cudaError_t e, const char* what) {
+  TORCH_CHECK(e == cudaSuccess, "glm53 kernel ", what, " failed: ", cudaGetErrorString(e));
+}
+cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+// numbers in messages are formatted here: streaming one into a string stream crashes in the process when the extension is
+// built with a C++ library that differs from the one torch loaded
+std::string num(int64_t v) { return std::to_string(v); }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// a 4-bit matrix: its arrays and shape, checked once when it is made
+struct Matrix4 {
+  Tensor codes, scales;
+  OptT row_scale;
+  int64_t rows, k;
+  bool nv;
+
+  Matrix4(Tensor c, Tensor s, OptT r, int64_t rows_, int64_t k_, bool nv_)
+      : codes(std::move(c)), scales(std::move(s)), row_scale(std::move(r)), rows(rows_), k(k_), nv(nv_) {
+    const int64_t block = nv ? 16 : 32;
+    TORCH_CHECK(rows >= 1 && k >= block && k % block == 0, "Matrix4: rows >= 1 and K a multiple of ", num(block), ", got [",
+                num(rows), ", ", num(k), "]");
+    TORCH_CHECK(rows < (int64_t)1 << 31 && k < (int64_t)1 << 31, "Matrix4: at most 2^31 - 1 rows and columns");
+    const int64_t tiles = ((rows + kTileRows - 1) / kTileRows) * ((k + kTileK - 1) / kTileK);
+    TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kByte && codes.is_contiguous() &&
+                    codes.numel() == tiles * kTileBytes && aligned16(codes.data_ptr()),
+                "Matrix4: codes must be ", num(tiles * kTileBytes), " contiguous, 16-byte aligned uint8 on a CUDA device");
+    TORCH_CHECK(scales.device() == codes.device() && scales.scalar_type() == at::kByte && scales.is_contiguous() &&
+                    scales.numel() == tiles * kTileRows * (kTileK / block) && aligned16(scales.data_ptr()),
+                "Matrix4: scales must be ", num(tiles * kTileRows * (kTileK / block)),
+                " contiguous, 16-byte aligned uint8 on the codes' device");
+    TORCH_CHECK(nv == row_scale.has_value(), "Matrix4: nvfp4 has a row scale, mxfp4 none");
+    if (nv)
+      TORCH_CHECK(row_scale->device() == codes.device() && row_scale->scalar_type() == at::kFloat &&
+                      row_scale->is_contiguous() && row_scale->numel() >= rows && aligned16(row_scale->data_ptr()),
+                  "Matrix4: row_scale must be fp32 [rows], contiguous, 16-byte aligned, on the codes' device");
+  }
+  const uint8_t* c() const { return codes.data_ptr<uint8_t>(); }
+  const uint8_t* s() const { return scales.data_ptr<uint8_t>(); }
+  const float* r() const { return nv ? row_scale->data_ptr<float>() : nullptr; }
+};
+
+Matrix4 empty4(int64_t rows, int64_t k, bool nv, const Tensor& like) {
+  const int64_t block = nv ? 16 : 32;
+  const int64_t tiles = ((rows + kTileRows - 1) / kTileRows) * ((k + kTileK - 1) / kTileK);
+  const auto u8 = like.options().dtype(at::kByte);
+  Tensor c = torch::empty({tiles * kTileBytes}, u8), s = torch::empty({tiles * kTileRows * (kTileK / block)}, u8);
+  OptT r;
+  if (nv) r = torch::empty({rows}, like.options().dtype(at::kFloat));
+  return Matrix4(std::move(c), std::move(s), std::move(r), rows, k, nv);
+}
+
+void check_x(const Tensor& x, const char* op) {
+  TORCH_CHECK(x.is_cuda(), op, ": x must be a CUDA tensor");
+  TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1), op, ": x must be [rows, K] with unit inner stride");
+  TORCH_CHECK(x.size(0) < (int64_t)1 << 31, op, ": at most 2^31 - 1 rows");
+}
+
+Matrix4 quantize(const Tensor& x, bool nv) {
+  check_x(x, "quantize4");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "quantize4: x must be bf16 or f16");
+  const c10::cuda::CUDAGuard guard(x.device());
+  Matrix4 m = empty4(x.size(0), x.size(1), nv, x);
+  Fp4QuantArgs a{};
+  a.x = x.data_ptr();
+  a.ldx = x.stride(0);
+  a.R = m.rows;
+  a.K = m.k;
+  a.nv = nv;
+  a.f16 = x.scalar_type() == at::kHalf;
+  a.vec = aligned16(a.x) && a.ldx % 8 == 0;
+  a.codes = m.codes.data_ptr<uint8_t>();
+  a.scales = m.scales.data_ptr<uint8_t>();
+  a.row_scale = nv ? m.row_scale->data_ptr<float>() : nullptr;
+  ok(g53_fp4_quantize(a, stream()), "fp4_quantize");
+  return m;
+}
+
+void dequant(const Matrix4& m, const Tensor& y, int64_t il) {
+  Fp4DequantArgs a{};
+  a.codes = m.c();
+  a.scales = m.s();
+  a.row_scale = m.r();
+  a.R = m.rows;
+  a.K = m.k;
+  a.nv = m.nv;
+  a.out = y.scalar_type() == at::kBFloat16 ? 0 : y.scalar_type() == at::kHalf ? 1 : 2;
+  a.il = il;
+  a.y = y.data_ptr();
+  a.ldy = y.stride(0);
+  a.vec = aligned16(a.y) && (a.ldy * y.element_size()) % 16 == 0;
+  ok(g53_fp4_dequant(a, stream()), "fp4_dequant");
+}
+
+void dequantize(const Matrix4& m, const Tensor& y) {
+  TORCH_CHECK(y.device() == m.codes.device(), "dequantize4: the output must be on the matrix's device");
+  TORCH_CHECK(y.scalar_type() == at::kBFloat16 || y.scalar_type() == at::kHalf || y.scalar_type() == at::kFloat,
+              "dequantize4: the output must be bf16, f16 or fp32");
+  TORCH_CHECK(y.dim() == 2 && y.size(0) == m.rows && y.size(1) == m.k && y.stride(1) == 1 &&
+                  (m.rows == 1 || y.stride(0) >= m.k),
+              "dequantize4: the output must be [", num(m.rows), ", ", num(m.k), "], rows contiguous and apart");
+  const c10::cuda::CUDAGuard guard(y.device());
+  dequant(m, y, 0);
+}
+
+void check_xy(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t mode, const char* op) {
+  check_x(x, op);
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16, op, ": x must be bf16");
+  TORCH_CHECK(x.device() == w.codes.device() && y.device() == x.device(), op, ": x, y and the weights must be on one device");
+  TORCH_CHECK(x.size(1) == w.k, op, ": K mismatch: x ", num(x.size(1)), ", weights ", num(w.k));
+  TORCH_CHECK(mode == GEMV_BF16 || mode == GEMV_F32 || mode == GEMV_F32_ACC, op, ": mode must be GEMV_BF16, GEMV_F32 or "
+              "GEMV_F32_ACC");
+  TORCH_CHECK(y.scalar_type() == (mode == GEMV_BF16 ? at::kBFloat16 : at::kFloat), op,
+              ": y must be bf16 (GEMV_BF16) or fp32 (the other modes)");
+  TORCH_CHECK(y.dim() == 2 && y.size(0) == x.size(0) && y.size(1) == n && (y.stride(1) == 1 || n == 1) &&
+                  (y.size(0) <= 1 || y.stride(0) >= n),
+              op, ": y must be [", num(x.size(0)), ", ", num(n), "], rows contiguous and apart");
+}
+
+// rows [m0, m0 + m) of x through the small-M kernel
+void gemv(const Tensor& x, int64_t m0, int64_t m, const Matrix4& w, const Tensor& y, int64_t n, int64_t width,
+          int64_t mode, double limit) {
+  Fp4GemvArgs a{};
+  a.x = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()) + m0 * x.stride(0);
+  a.ldx = x.stride(0);
+  a.xvec = aligned16(a.x) && a.ldx % 8 == 0;
+  a.codes = w.c();
+  a.scales = w.s();
+  a.row_scale = w.r();
+  a.nv = w.nv;
+  a.y = reinterpret_cast<uint8_t*>(y.data_ptr()) + m0 * y.stride(0) * y.element_size();
+  a.ldy = y.stride(0);
+  a.M = (int)m;
+  a.N = (int)n;
+  a.K = (int)w.k;
+  a.width = (int)width;
+  a.mode = (int)mode;
+  a.limit = (float)limit;
+  ok(g53_fp4_gemv(a, stream()), "fp4_gemv");
+}
+
+// exact activations, many rows: the weights widened to bf16 (every 4-bit value times its scales is a bf16 value), then
+// the bf16 tcgen05 GEMM
+void gemm_exact(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t il, int64_t mode, double limit) {
+  Tensor xx = aligned16(x.data_ptr()) && x.stride(0) % 8 == 0 ? x : x.contiguous().clone();
+  Tensor wb = torch::empty({n, w.k}, x.options());
+  dequant(w, wb, il);
+  GemmArgs p{};
+  p.a = xx.data_ptr();
+  p.lda = xx.stride(0);
+  p.b = wb.data_ptr();
+  p.ldb = wb.stride(0);
+  p.y = y.data_ptr();
+  p.ldy = y.stride(0);
+  p.M = (int)x.size(0);
+  p.N = (int)n;
+  p.K = (int)w.k;
+  p.mode = (int)mode;
+  p.limit = (float)limit;
+  ok(g53_fp4_gemm_error_word(&p.err), "fp4 error word");
+  ok(g53_gemm_sm100(p, stream()), "gemm_sm100");
+}
+
+Fp4GemmArgs gemm_args(const Matrix4& a, const Matrix4& w, int64_t mode) {
+  Fp4GemmArgs p{};
+  p.a_codes = a.c();
+  p.a_scales = a.s();
+  p.a_row = a.r();
+  p.a_const = 1.f;
+  p.b_codes = w.c();
+  p.b_scales = w.s();
+  p.b_row = w.r();
+  p.nv = w.nv;
+  p.M = (int)a.rows;
+  p.N = (int)w.rows;
+  p.K = (int)w.k;
+  p.mode = (int)mode;
+  return p;
+}
+
+void linear(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t mode, bool act4) {
+  check_xy(x, w, y, w.rows, mode, "linear4");
+  const int64_t M = x.size(0);
+  if (M == 0) return;
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (M > kGemvRows && act4) {
+    const Matrix4 a = quantize(x, w.nv);
+    Fp4GemmArgs p = gemm_args(a, w, mode);
+    p.y = y.data_ptr();
+    p.ldy = y.stride(0);
+    ok(g53_fp4_gemm(p, stream()), "fp4_gemm");
+  } else if (M >= kGemmRows) {
+    gemm_exact(x, w, y, w.rows, 0, mode, 0.0);
+  } else {
+    for (int64_t m = 0; m < M; m += kGemvRows) gemv(x, m, std::min(kGemvRows, M - m), w, y, w.rows, 0, mode, 0.0);
+  }
+}
+
+// smallest k with bound <= 448 * 6 * 2^k (fp4.cuh: nv_row_exp)
+int row_exp(float bound) {
+  uint32_t b;
+  std::memcpy(&b, &bound, 4);
+  const int k = (int)(b >> 23) - 127 - 11 + ((b & 0x7fffffu) > 0x280000u ? 1 : 0);
+  return std::max(k, -126);
+}
+
+void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& y, double limit, int64_t mode, bool act4) {
+  const int64_t W = down.k;
+  TORCH_CHECK(gu.nv == down.nv && gu.codes.device() == down.codes.device(), "mlp4: both matrices in one format, on one device");
+  TORCH_CHECK(W % 32 == 0 && gu.rows == (W + 63) / 64 * 128, "mlp4: the gate/up image must have ", num((W + 63) / 64 * 128),
+              " rows for a width of ", num(W), " (a multiple of 32)");
+  check_xy(x, gu, y, down.rows, mode, "mlp4");
+  TORCH_CHECK(limit > 0, "mlp4: limit must be positive (infinity: no clamp)");
+  const int64_t M = x.size(0);
+  const float l2 = (float)limit * (float)limit;
+  const bool four = act4 && M > kGemvRows;
+  TORCH_CHECK(!four || !gu.nv || (std::isfinite(l2) && l2 >= 1e-30f),
+              "mlp4: 4-bit nvfp4 activations need a finite limit (their row scale comes from it)");
+  if (M == 0) return;
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (four) {
+    const Matrix4 a = quantize(x, gu.nv);
+    Matrix4 h = empty4(M, W, gu.nv, x);
+    Fp4GemmArgs p = gemm_args(a, gu, GEMV_SWIGLU);
+    p.limit = (float)limit;
+    p.width = (int)W;
+    p.out_codes = h.codes.data_ptr<uint8_t>();
+    p.out_scales = h.scales.data_ptr<uint8_t>();
+    p.h_exp = gu.nv ? row_exp(l2) : 0;
+    ok(g53_fp4_gemm(p, stream()), "fp4_gemm");
+    Fp4GemmArgs d = gemm_args(h, down, mode);
+    d.a_row = nullptr;
+    d.a_const = gu.nv ? std::ldexp(1.f, p.h_exp) : 1.f;
+    d.y = y.data_ptr();
+    d.ldy = y.stride(0);
+    ok(g53_fp4_gemm(d, stream()), "fp4_gemm");
+    return;
+  }
+  const Tensor h = torch::empty({M, W}, x.options());
+  if (M >= kGemmRows) {
+    gemm_exact(x, gu, h, 2 * W, W, GEMV_SWIGLU_F32, limit);
+    gemm_exact(h, down, y, down.rows, 0, mode, 0.0);
+    return;
+  }
+  for (int64_t m = 0; m < M; m += kGemvRows) gemv(x, m, std::min(kGemvRows, M - m), gu, h, gu.rows, W, GEMV_SWIGLU, limit);
+  for (int64_t m = 0; m < M; m += kGemvRows) gemv(h, m, std::min(kGemvRows, M - m), down, y, down.rows, 0, mode, 0.0);
+}
+
+int64_t error(int64_t device) {
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  int a = 0, b = 0;
+  ok(g53_fp4_gemv_error(&a), "fp4_gemv_error");
+  ok(g53_fp4_gemm_error(&b), "fp4_gemm_error");
+  return a ? a : b;
+}
+
+}  // namespace
+
+void register_fp4(pybind11::module& m) {
+  namespace py = pybind11;
+  py::class_<Matrix4>(m, "Matrix4")
+      .def(py::init<Tensor, Tensor, OptT, int64_t, int64_t, bool>())
+      .def_readonly("codes", &Matrix4::codes)
+      .def_readonly("scales", &Matrix4::scales)
+      .def_readonly("row_scale", &Matrix4::row_scale)
+      .def_readonly("rows", &Matrix4::rows)
+      .def_readonly("k", &Matrix4::k)
+      .def_readonly("nv", &Matrix4::nv);
+  m.def("fp4_quantize", &quantize);
+  m.def("fp4_dequantize", &dequantize);
+  m.def("fp4_linear", &linear);
+  m.def("fp4_mlp", &mlp);
+  m.def("fp4_error", &error);
+}

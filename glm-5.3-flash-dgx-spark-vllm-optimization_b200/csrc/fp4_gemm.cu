@@ -1,0 +1,442 @@
+// Large-M product of two 4-bit matrices on the block-scaled tensor cores: Y[M, N] = A4[M, K] @ W4[N, K]^T (W4A4).
+//
+// tcgen05.mma kind::mxf4nvf4 (nvfp4: scale_vec::4X, one e4m3 scale per 16) and kind::mxf4 (mxfp4: scale_vec::2X, one E8M0
+// scale per 32): the tensor core multiplies e2m1 codes, applies both block scales and sums in fp32, at four times the
+// bf16 rate.  Row scales (nvfp4) are applied to the fp32 result.
+//
+// Persistent, one CTA per SM, output tiles of 128 x BN in bands of 8 row blocks.  Both operands are tile images (fp4.cuh),
+// so a K step of 256 is one contiguous cp.async.bulk per 128-row block and array, already swizzled.  Warp roles:
+//   warp 0    producer: fills a 4-stage (BN 256) ring, continuously across tiles
+//   warp 1    allocates TMEM; one thread copies the block scales of the stage to TMEM (tcgen05.cp, executed in order with
+//             the mma of the same thread) and issues the four K = 64 mma of the stage
+//   warps 2-5 epilogue: tcgen05.ld, row scales, output
+// TMEM (512 columns): scales at 448..495; with BN = 256 the two accumulators are columns 0..255 and 192..447.  They share
+// 64 columns, which the epilogue of a tile reads first and then hands back, so the main loop of the next tile waits
+// for a quarter of the epilogue's loads only.
+//
+// GEMV_SWIGLU: W4 is a gate/up image (per 128-row block 64 gate rows, then their 64 up rows); the epilogue forms
+// silu(min(g, L)) * clip(u, -L, L) in fp32 and quantises it in place: a thread holds 32 consecutive activations of one row,
+// a whole 16-byte chunk of the 4-bit image that the down projection reads.  The nvfp4 row scale cannot wait for the row's
+// maximum (other CTAs hold the rest of the row), so it is the one that fits L * L, the largest possible activation; the
+// e4m3 block scales then have 2^15 of range below it.
+//
+// Waits are bounded; a timeout sets the error word, the roles stop issuing, wait for what they have in flight, and the
+// TMEM is freed.
+#include <algorithm>
+#include "fp4.cuh"
+#include "launchers.h"
+#include "tc05.cuh"
+
+namespace g53 {
+namespace fp4 {
+
+__device__ int g_gemm_err = 0;
+
+constexpr int kGemmThreads = 192;
+constexpr int kBandM = 8;
+constexpr uint32_t kSfA = 448, kSfB = 464;            // TMEM columns of the scales
+
+template <bool NV, int BN>
+struct GemmCfg {
+  static constexpr int kNB = BN / 128;                // 128-row blocks of W per tile
+  static constexpr int kSB = Fmt<NV>::kScaleBytes;
+  static constexpr int kAtoms = kSB / 512;            // scale atoms per block and stage
+  static constexpr int kStage = (1 + kNB) * (kTileBytes + kSB);
+  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr int kSmem = kStages * kStage + 1024;
+  static constexpr uint32_t kBuf = BN == 256 ? 192 : 128;   // column of the second accumulator
+};
+
+// instruction descriptor of the 4-bit block-scaled kinds: A, B e2m1, K-major; scale type (0 e4m3, 1 E8M0); M; N; scale
+// data ids (which half of a 32-bit scale column the mma uses: 2X only)
+__device__ __forceinline__ uint32_t idesc4(int m, int n, bool ue8m0, uint32_t sf_id) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
+         ((uint32_t)(m >> 7) << 27) | (sf_id << 29);
+}
+
+template <bool NV>
+__device__ __forceinline__ void mma4(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t sfa, uint32_t sfb,
+                                     uint32_t acc) {
+  if constexpr (NV) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"(acc));
+  } else {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"(acc));
+  }
+}
+
+// one scale atom (32 rows x 16 bytes) -> 4 TMEM columns, repeated in the four lane quadrants.  Descriptor: no swizzle,
+// 8-row groups 128 bytes apart
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
+  uint64_t d = (uint64_t)((smem >> 4) & 0x3FFF);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(128 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d));
+}
+
+__device__ __forceinline__ void gm_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(tc::saddr(dst)), "l"(src), "r"(bytes), "r"(tc::saddr(bar)) : "memory");
+}
+__device__ __forceinline__ void gm_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::saddr(b)), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void tile_mn(int t, int MT, int NT, int& m, int& n) {
+  const int band = t / (kBandM * NT);
+  const int gm = min(kBandM, MT - band * kBandM);
+  const int idx = t - band * kBandM * NT;
+  m = band * kBandM + idx % gm;
+  n = idx / gm;
+}
+
+// 32 columns nb.. of one row
+__device__ __forceinline__ void store32(const Fp4GemmArgs& p, int row, int nb, float rs, float (&v)[32]) {
+  const bool full = nb + 32 <= p.N;
+  if (p.b_row) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      if (full) {
+        const float4 t = *reinterpret_cast<const float4*>(p.b_row + nb + i);
+        v[i] *= rs * t.x; v[i + 1] *= rs * t.y; v[i + 2] *= rs * t.z; v[i + 3] *= rs * t.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (nb + i + j < p.N) v[i + j] *= rs * p.b_row[nb + i + j];
+      }
+    }
+  }
+  const int64_t off = (int64_t)row * p.ldy + nb;
+  if (p.mode == GEMV_BF16) {
+    __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + off;
+    if (full && p.vec) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          __nv_bfloat162 b = __floats2bfloat162_rn(v[c * 8 + 2 * i], v[c * 8 + 2 * i + 1]);
+          w[i] = *reinterpret_cast<uint32_t*>(&b);
+        }
+        reinterpret_cast<uint4*>(y)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (nb + i < p.N) y[i] = f2bf(v[i]);
+    }
+    return;
+  }
+  float* y = reinterpret_cast<float*>(p.y) + off;
+  const bool acc = p.mode == GEMV_F32_ACC;
+  if (full && p.vec) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      float4 o = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+      if (acc) {
+        const float4 t = reinterpret_cast<const float4*>(y)[c];
+        o.x += t.x; o.y += t.y; o.z += t.z; o.w += t.w;
+      }
+      reinterpret_cast<float4*>(y)[c] = o;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (nb + i < p.N) y[i] = acc ? y[i] + v[i] : v[i];
+  }
+}
+
+// 32 activations j0.. of one row: gate (v) and up (u) sums -> 4-bit chunk and block scales of the output image
+template <bool NV>
+__device__ __forceinline__ void swiglu32(const Fp4GemmArgs& p, int row, int j0, int r0, float rs, float (&v)[32],
+                                         float (&u)[32]) {
+  const float L = p.limit;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    float g = v[i], w = u[i];
+    if constexpr (NV) {
+      g *= rs * p.b_row[r0 + i];
+      w *= rs * p.b_row[r0 + 64 + i];
+    }
+    g = g > L ? L : g;                                // written so that a NaN stays one
+    w = w > L ? L : w < -L ? -L : w;
+    v[i] = siluf_(g) * w;
+  }
+  const int rr = row % kTileRows, kt = j0 / kTileK, c = (j0 % kTileK) / 32;
+  const int64_t tile = (int64_t)(row / kTileRows) * tiles_k(p.width) + kt;
+  uint32_t code[4];
+  uint32_t sc = 0;
+  if constexpr (NV) {
+    const float down = pow2i(-p.h_exp);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t am = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) am = max(am, __float_as_uint(v[h * 16 + i]) & 0x7fffffffu);
+      const uint32_t b = am >= kInfBits ? 0x7fu : nv_scale(__uint_as_float(am) * down);
+      const float s = e4m3_to_f32(b);
+      const float inv = s > 0.f ? __frcp_rn(s) * down : 0.f;
+      sc |= b << (8 * h);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = v[h * 16 + k * 8 + i] * inv;
+        code[h * 2 + k] = f32x8_to_e2m1(f);
+      }
+    }
+    *reinterpret_cast<uint16_t*>(p.out_scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, 2 * c)) = (uint16_t)sc;
+  } else {
+    uint32_t am = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) am = max(am, __float_as_uint(v[i]) & 0x7fffffffu);
+    sc = mx_scale(am);
+    const float inv = sc == 255u ? 0.f : pow2i(127 - (int)sc);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = v[k * 8 + i] * inv;
+      code[k] = f32x8_to_e2m1(f);
+    }
+    p.out_scales[tile * Fmt<NV>::kScaleBytes + scale_off(rr, c)] = (uint8_t)sc;
+  }
+  *reinterpret_cast<uint4*>(p.out_codes + tile * kTileBytes + chunk_off(rr, c)) =
+      make_uint4(code[0], code[1], code[2], code[3]);
+}
+
+template <bool NV, int BN, bool SWI>
+__global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p) {
+  using C = GemmCfg<NV, BN>;
+  constexpr int kStages = C::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], drain;
+  __shared__ uint32_t tmem_s;
+  __shared__ int fail_s;
+  volatile int* fail = &fail_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int KT = tiles_k(p.K);
+  const int ksteps = (p.K + 63) / 64;
+  const int MT = (p.M + 127) / 128, NB = (p.N + 127) / 128, NT = (NB + C::kNB - 1) / C::kNB;
+  const int tiles = MT * NT;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      tc::bar_init(&full[s], 1);
+      tc::bar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      tc::bar_init(&tfull[b], 1);
+      tc::bar_init(&tempty[b], 4);
+    }
+    tc::bar_init(&drain, 1);
+    fail_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tc::tmem_alloc(&tmem_s, 512);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_s;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        int mb, nt;
+        tile_mn(t, MT, NT, mb, nt);
+        const int nblk = min(C::kNB, NB - nt * C::kNB);
+        for (int kt = 0; kt < KT; ++kt, ++it) {
+          const int s = it % kStages;
+          if (it >= kStages && !tc::bar_wait(&empty[s], ((it / kStages) - 1) & 1, fail, &g_gemm_err, 1)) {
+            ok = false;
+            break;
+          }
+          uint8_t* a = smem + s * C::kStage;
+          uint8_t* sa = a + (1 + C::kNB) * kTileBytes;
+          gm_expect(&full[s], (uint32_t)(1 + nblk) * (kTileBytes + C::kSB));
+          const int64_t ta = (int64_t)mb * KT + kt;
+          gm_bulk(a, p.a_codes + ta * kTileBytes, kTileBytes, &full[s]);
+          gm_bulk(sa, p.a_scales + ta * C::kSB, C::kSB, &full[s]);
+          for (int b = 0; b < nblk; ++b) {
+            const int64_t tb = (int64_t)(nt * C::kNB + b) * KT + kt;
+            gm_bulk(a + (1 + b) * kTileBytes, p.b_codes + tb * kTileBytes, kTileBytes, &full[s]);
+            gm_bulk(sa + (1 + b) * C::kSB, p.b_scales + tb * C::kSB, C::kSB, &full[s]);
+          }
+        }
+      }
+      if (*fail) {
+        const uint32_t first = it > (uint32_t)kStages ? it - kStages : 0;
+        int none = 0;
+        for (uint32_t j = first; j < it; ++j) tc::bar_wait(&full[j % kStages], (j / kStages) & 1, &none, nullptr, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t it = 0, tl = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++tl) {
+        const uint32_t buf = tl & 1;
+        // BN 256: the shared columns of the tile before; BN 128: the buffer's last tile
+        const uint32_t lag = BN == 256 ? 1 : 2;
+        if (tl >= lag && !tc::bar_wait(&tempty[(tl - lag) & 1], ((tl - lag) >> 1) & 1, fail, &g_gemm_err, 4)) break;
+        tc::fence_after();
+        const uint32_t d = tmem + buf * C::kBuf;
+        for (int kt = 0; kt < KT; ++kt, ++it) {
+          const int s = it % kStages;
+          if (!tc::bar_wait(&full[s], (it / kStages) & 1, fail, &g_gemm_err, 2)) {
+            ok = false;
+            break;
+          }
+          tc::fence_after();
+          const uint32_t a = tc::saddr(smem + s * C::kStage);
+          const uint32_t b = a + kTileBytes;
+          const uint32_t sa = a + (1 + C::kNB) * kTileBytes;
+#pragma unroll
+          for (int at = 0; at < C::kAtoms; ++at) {
+            copy_scales(tmem + kSfA + at * 4, sa + at * 512);
+#pragma unroll
+            for (int nb = 0; nb < C::kNB; ++nb)
+              copy_scales(tmem + kSfB + at * (4 * C::kNB) + nb * 4, sa + (1 + nb) * C::kSB + at * 512);
+          }
+          const int n = min(4, ksteps - kt * 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k >= n) break;
+            const int at = NV ? k : k >> 1;
+            const uint32_t sf = NV ? 0u : (uint32_t)(k & 1) * 2;
+            mma4<NV>(d, tc::desc_sw128(a + k * 32), tc::desc_sw128(b + k * 32), idesc4(128, BN, !NV, sf),
+                     tmem + kSfA + at * 4, tmem + kSfB + at * (4 * C::kNB), (kt > 0 || k > 0) ? 1u : 0u);
+          }
+          tc::commit(&empty[s]);
+        }
+        if (ok) tc::commit(&tfull[buf]);
+      }
+      if (*fail) {
+        int none = 0;
+        tc::commit(&drain);
+        tc::bar_wait(&drain, 0, &none, nullptr, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quad = warp & 3;
+    uint32_t tl = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++tl) {
+      const uint32_t buf = tl & 1;
+      int mb, nt;
+      tile_mn(t, MT, NT, mb, nt);
+      if (!tc::warp_wait(&tfull[buf], (tl >> 1) & 1, fail, &g_gemm_err, 3)) break;
+      tc::fence_after();
+      const int row = mb * 128 + quad * 32 + lane;
+      const bool live = row < p.M;
+      const float rs = p.a_row && live ? p.a_row[row] : p.a_const;
+      const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + buf * C::kBuf;
+      auto release = [&]() {
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::bar_arrive(&tempty[buf]);
+      };
+      // units of 64 columns; the one in the shared columns first
+      if constexpr (SWI) {
+#pragma unroll 1
+        for (int i = 0; i < C::kNB; ++i) {
+          const int blk = C::kNB == 2 ? (buf == 0 ? 1 - i : i) : 0;
+          const int nblk = nt * C::kNB + blk;
+          // the half of the pair that lies in the shared columns: up (buffer 0, block 1) or gate (buffer 1, block 0)
+          const uint32_t first = buf == 0 ? 64u : 0u;
+          float x0[32], x1[32], w[32];
+          tc::tmem_ld32(base + blk * 128 + first, x0);
+          tc::tmem_ld32(base + blk * 128 + first + 32, x1);
+          if (C::kNB == 2 && i == 0) release();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            tc::tmem_ld32(base + blk * 128 + (64u - first) + h * 32, w);
+            const int j0 = nblk * 64 + h * 32;
+            if (live && j0 < ((p.width + 63) / 64) * 64) {
+              const int r0 = nblk * 128 + h * 32;
+              if (buf == 0) swiglu32<NV>(p, row, j0, r0, rs, w, h == 0 ? x0 : x1);
+              else swiglu32<NV>(p, row, j0, r0, rs, h == 0 ? x0 : x1, w);
+            }
+          }
+          if (C::kNB == 1) release();
+        }
+      } else {
+        const int n0 = nt * BN;
+#pragma unroll 1
+        for (int i = 0; i < BN / 64; ++i) {
+          const int u = BN == 256 && buf == 0 ? (i + 3) & 3 : i;
+          float x0[32], x1[32];
+          tc::tmem_ld32(base + u * 64, x0);
+          tc::tmem_ld32(base + u * 64 + 32, x1);
+          if (BN == 256 ? i == 0 : i == BN / 64 - 1) release();
+          if (live && n0 + u * 64 < p.N) store32(p, row, n0 + u * 64, rs, x0);
+          if (live && n0 + u * 64 + 32 < p.N) store32(p, row, n0 + u * 64 + 32, rs, x1);
+        }
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after();
+    tc::tmem_free(tmem, 512);
+  }
+}
+
+template <bool NV, int BN, bool SWI>
+static cudaError_t launch_gemm(const Fp4GemmArgs& p, int sms, cudaStream_t st) {
+  using C = GemmCfg<NV, BN>;
+  auto kern = fp4_gemm_kernel<NV, BN, SWI>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + BN - 1) / BN);
+  kern<<<(unsigned)std::min<int64_t>(tiles, sms), kGemmThreads, C::kSmem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <bool NV>
+static cudaError_t gemm_t(const Fp4GemmArgs& p, int sms, cudaStream_t st) {
+  const bool wide = (int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256) >= sms;
+  if (p.mode == GEMV_SWIGLU)
+    return wide ? launch_gemm<NV, 256, true>(p, sms, st) : launch_gemm<NV, 128, true>(p, sms, st);
+  return wide ? launch_gemm<NV, 256, false>(p, sms, st) : launch_gemm<NV, 128, false>(p, sms, st);
+}
+
+}  // namespace fp4
+}  // namespace g53
+
+using namespace g53;
+
+cudaError_t g53_fp4_gemm(const Fp4GemmArgs& p, cudaStream_t st) {
+  if (p.M < 1 || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  Fp4GemmArgs q = p;
+  const int esz = p.mode == GEMV_BF16 ? 2 : 4;
+  q.vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && ((p.ldy * esz) & 15) == 0 ? 1 : 0;
+  return p.nv ? fp4::gemm_t<true>(q, sms, st) : fp4::gemm_t<false>(q, sms, st);
+}
+
+cudaError_t g53_fp4_gemm_error_word(int** word) {
+  return cudaGetSymbolAddress(reinterpret_cast<void**>(word), fp4::g_gemm_err);
+}
+
+cudaError_t g53_fp4_gemm_error(int* code) {
+  const int z = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(code, fp4::g_gemm_err, sizeof(int));
+  if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(fp4::g_gemm_err, &z, sizeof(int));
+  return e;
+}

@@ -7,7 +7,9 @@
 #include <stdint.h>
 
 // ---------------------------------------------------------------- small-M GEMM (gemv.cu)
-enum GemvMode { GEMV_BF16 = 0, GEMV_F32 = 1, GEMV_F32_ACC = 2, GEMV_SWIGLU = 3 };
+// GEMV_SWIGLU rounds gate and up to bf16 before the activation; GEMV_SWIGLU_F32 (gemm_sm100.cu) keeps them in fp32 and
+// lets a NaN through the clamps
+enum GemvMode { GEMV_BF16 = 0, GEMV_F32 = 1, GEMV_F32_ACC = 2, GEMV_SWIGLU = 3, GEMV_SWIGLU_F32 = 4 };
 
 struct GemvArgs {
   const __nv_bfloat16* x; int64_t ldx; int64_t bsx;   // activations [batch][M][K] (row stride ldx)
@@ -390,3 +392,58 @@ struct RejectArgs {
   float* scratch;              // [B, K+1] block acceptance stats
 };
 cudaError_t g53_rejection_sample(const RejectArgs& a, cudaStream_t st);
+
+// ---------------------------------------------------------------- 4-bit floating point (fp4_*.cu, layout in fp4.cuh)
+struct Fp4QuantArgs {
+  const void* x; int64_t ldx;          // [R, K] bf16 or f16 rows, unit inner stride
+  int64_t R, K;
+  int nv, f16;                         // nvfp4 (else mxfp4); input f16 (else bf16)
+  int vec;                             // 16-byte aligned rows
+  uint8_t* codes; uint8_t* scales; float* row_scale;
+};
+cudaError_t g53_fp4_quantize(const Fp4QuantArgs& p, cudaStream_t st);
+
+struct Fp4DequantArgs {
+  const uint8_t* codes; const uint8_t* scales; const float* row_scale;
+  int64_t R, K;
+  int nv, out;                         // out: 0 bf16, 1 f16, 2 fp32
+  int vec;                             // 16-byte aligned output rows
+  int64_t il;                          // > 0: gate/up image of this width, rows written in the (8 gate, 8 up) interleave
+  void* y; int64_t ldy;
+};
+cudaError_t g53_fp4_dequant(const Fp4DequantArgs& p, cudaStream_t st);
+
+// y[M, N] (mode) = x[M, K] bf16 @ W4[N, K]^T, M <= 16 (fp4_gemv.cu).  GEMV_SWIGLU: W4 is a gate/up image (64 gate rows,
+// then their 64 up rows, per 128-row block), y [M, width] bf16
+struct Fp4GemvArgs {
+  const __nv_bfloat16* x; int64_t ldx; int xvec;
+  const uint8_t* codes; const uint8_t* scales; const float* row_scale;
+  int nv;
+  void* y; int64_t ldy;
+  int M, N, K;
+  int width;                           // GEMV_SWIGLU: columns of y
+  int mode;
+  float limit;
+};
+cudaError_t g53_fp4_gemv(const Fp4GemvArgs& p, cudaStream_t st);
+
+// y[M, N] (mode) = A4[M, K] @ W4[N, K]^T on the block-scaled tensor-core path (fp4_gemm.cu).  out_* (GEMV_SWIGLU): the
+// activations are written as a 4-bit image [M, width] with the row scale 2^h_exp (nvfp4)
+struct Fp4GemmArgs {
+  const uint8_t* a_codes; const uint8_t* a_scales; const float* a_row; float a_const;   // a_row null: a_const
+  const uint8_t* b_codes; const uint8_t* b_scales; const float* b_row;
+  int nv;
+  void* y; int64_t ldy;
+  int M, N, K;
+  int mode;
+  float limit;
+  int width;
+  uint8_t* out_codes; uint8_t* out_scales; int h_exp;
+  int vec;                             // set by the launcher: 16-byte epilogue stores allowed
+};
+cudaError_t g53_fp4_gemm(const Fp4GemmArgs& p, cudaStream_t st);
+// the current device's error word of the large-M kernels (bounded waits)
+cudaError_t g53_fp4_gemm_error_word(int** word);
+// first error code recorded on the current device by a bounded wait of these kernels (0: none); clears it
+cudaError_t g53_fp4_gemv_error(int* code);
+cudaError_t g53_fp4_gemm_error(int* code);
