@@ -13,6 +13,8 @@
 //           the order tcgen05.cp.32x128b.warpx4 carries to TMEM: byte (r % 32) * 16 + (r / 32) * 4 + column % 4
 // Columns past K in the last tile hold zero codes and zero scales; rows past R are not written.
 #pragma once
+#include <cuda_fp4.h>
+
 #include "common.cuh"
 
 namespace g53 {
@@ -36,12 +38,15 @@ __device__ __forceinline__ int chunk_off(int r, int c) { return r * 128 + ((c ^ 
 // byte of block column s of row r inside a scale tile
 __device__ __forceinline__ int scale_off(int r, int s) { return (s >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (s & 3); }
 
-// 8 codes (one 32-bit word) -> four f16x2, exact; o[i] holds codes 2i (low half) and 2i + 1
+// 8 codes (one 32-bit word) -> four f16x2, exact; o[i] holds codes 2i (low half) and 2i + 1.  Through CUDA's function,
+// a byte at a time: an inline unpack of the word into four .b8 registers came out of the assembler (12.9) with bytes
+// exchanged or lost, depending on what stood before it.
 __device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&o)[4]) {
-  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
-      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
-      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}\n"
-      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((w >> (8 * i)) & 0xffu), __NV_E2M1);
+    o[i] = (uint32_t)h.x | ((uint32_t)h.y << 16);
+  }
 }
 // 8 values -> 8 codes (nearest, ties to even, saturating at 6)
 __device__ __forceinline__ uint32_t f32x8_to_e2m1(const float (&v)[8]) {

@@ -18,7 +18,8 @@ using at::Tensor;
 using OptT = c10::optional<Tensor>;
 
 constexpr int64_t kTileRows = 128, kTileK = 256, kTileBytes = 16384;
-constexpr int64_t kGemvRows = 16;      // rows of one small-M launch
+constexpr int64_t kFourRows = 16;      // rows above which act4 quantises the activations
+constexpr int64_t kSkinnyRows = 32;    // rows of one small-M launch
 constexpr int64_t kGemmRows = 64;      // rows from which exact activations go through the bf16 tcgen05 GEMM
 
 void ok(cudaError_t e, const char* what) {
@@ -139,26 +140,54 @@ void check_xy(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int
               op, ": y must be [", num(x.size(0)), ", ", num(n), "], rows contiguous and apart");
 }
 
-// rows [m0, m0 + m) of x through the small-M kernel
-void gemv(const Tensor& x, int64_t m0, int64_t m, const Matrix4& w, const Tensor& y, int64_t n, int64_t width,
-          int64_t mode, double limit) {
-  Fp4GemvArgs a{};
+// 4-bit expansion of some rows of x (scratch of one call)
+struct Expanded {
+  Tensor codes, scales, factor;
+  int M;
+};
+
+Expanded expand(const Tensor& x, int64_t m0, int64_t m, bool nv) {
+  const int64_t K = x.size(1), tiles = (m * g53_fp4_terms() + kTileRows - 1) / kTileRows * ((K + kTileK - 1) / kTileK);
+  const int64_t sb = kTileRows * (kTileK / (nv ? 16 : 32));
+  const Tensor buf = torch::empty({tiles * (kTileBytes + sb) + m * 4}, x.options().dtype(at::kByte));
+  Expanded e{buf.narrow(0, 0, tiles * kTileBytes), buf.narrow(0, tiles * kTileBytes, tiles * sb),
+             buf.narrow(0, tiles * (kTileBytes + sb), m * 4), (int)m};
+  Fp4ExpandArgs a{};
   a.x = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()) + m0 * x.stride(0);
   a.ldx = x.stride(0);
-  a.xvec = aligned16(a.x) && a.ldx % 8 == 0;
-  a.codes = w.c();
-  a.scales = w.s();
-  a.row_scale = w.r();
-  a.nv = w.nv;
-  a.y = reinterpret_cast<uint8_t*>(y.data_ptr()) + m0 * y.stride(0) * y.element_size();
-  a.ldy = y.stride(0);
   a.M = (int)m;
-  a.N = (int)n;
-  a.K = (int)w.k;
-  a.width = (int)width;
-  a.mode = (int)mode;
-  a.limit = (float)limit;
-  ok(g53_fp4_gemv(a, stream()), "fp4_gemv");
+  a.K = (int)K;
+  a.nv = nv;
+  a.vec = aligned16(a.x) && a.ldx % 8 == 0;
+  a.codes = e.codes.data_ptr<uint8_t>();
+  a.scales = e.scales.data_ptr<uint8_t>();
+  a.factor = reinterpret_cast<float*>(e.factor.data_ptr());
+  ok(g53_fp4_expand(a, stream()), "fp4_expand");
+  return e;
+}
+
+// all rows of x through the small-M kernel, kSkinnyRows at a time
+void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t width, int64_t mode, double limit) {
+  for (int64_t m0 = 0; m0 < x.size(0); m0 += kSkinnyRows) {
+    const Expanded e = expand(x, m0, std::min(kSkinnyRows, x.size(0) - m0), w.nv);
+    Fp4SkinnyArgs a{};
+    a.x_codes = e.codes.data_ptr<uint8_t>();
+    a.x_scales = e.scales.data_ptr<uint8_t>();
+    a.x_factor = reinterpret_cast<const float*>(e.factor.data_ptr());
+    a.codes = w.c();
+    a.scales = w.s();
+    a.row_scale = w.r();
+    a.nv = w.nv;
+    a.y = reinterpret_cast<uint8_t*>(y.data_ptr()) + m0 * y.stride(0) * y.element_size();
+    a.ldy = y.stride(0);
+    a.M = e.M;
+    a.N = (int)n;
+    a.K = (int)w.k;
+    a.width = (int)width;
+    a.mode = (int)mode;
+    a.limit = (float)limit;
+    ok(g53_fp4_skinny(a, stream()), "fp4_skinny");
+  }
 }
 
 // exact activations, many rows: the weights widened to bf16 (every 4-bit value times its scales is a bf16 value), then
@@ -205,7 +234,7 @@ void linear(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t mode, bo
   const int64_t M = x.size(0);
   if (M == 0) return;
   const c10::cuda::CUDAGuard guard(x.device());
-  if (M > kGemvRows && act4) {
+  if (M > kFourRows && act4) {
     const Matrix4 a = quantize(x, w.nv);
     Fp4GemmArgs p = gemm_args(a, w, mode);
     p.y = y.data_ptr();
@@ -214,7 +243,7 @@ void linear(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t mode, bo
   } else if (M >= kGemmRows) {
     gemm_exact(x, w, y, w.rows, 0, mode, 0.0);
   } else {
-    for (int64_t m = 0; m < M; m += kGemvRows) gemv(x, m, std::min(kGemvRows, M - m), w, y, w.rows, 0, mode, 0.0);
+    skinny(x, w, y, w.rows, 0, mode, 0.0);
   }
 }
 
@@ -235,7 +264,7 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
   TORCH_CHECK(limit > 0, "mlp4: limit must be positive (infinity: no clamp)");
   const int64_t M = x.size(0);
   const float l2 = (float)limit * (float)limit;
-  const bool four = act4 && M > kGemvRows;
+  const bool four = act4 && M > kFourRows;
   TORCH_CHECK(!four || !gu.nv || (std::isfinite(l2) && l2 >= 1e-30f),
               "mlp4: 4-bit nvfp4 activations need a finite limit (their row scale comes from it)");
   if (M == 0) return;
@@ -264,14 +293,14 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
     gemm_exact(h, down, y, down.rows, 0, mode, 0.0);
     return;
   }
-  for (int64_t m = 0; m < M; m += kGemvRows) gemv(x, m, std::min(kGemvRows, M - m), gu, h, gu.rows, W, GEMV_SWIGLU, limit);
-  for (int64_t m = 0; m < M; m += kGemvRows) gemv(h, m, std::min(kGemvRows, M - m), down, y, down.rows, 0, mode, 0.0);
+  skinny(x, gu, h, gu.rows, W, GEMV_SWIGLU, limit);
+  skinny(h, down, y, down.rows, 0, mode, 0.0);
 }
 
 int64_t error(int64_t device) {
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   int a = 0, b = 0;
-  ok(g53_fp4_gemv_error(&a), "fp4_gemv_error");
+  ok(g53_fp4_skinny_error(&a), "fp4_skinny_error");
   ok(g53_fp4_gemm_error(&b), "fp4_gemm_error");
   return a ? a : b;
 }

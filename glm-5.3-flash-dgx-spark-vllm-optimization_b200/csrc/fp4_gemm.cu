@@ -24,8 +24,8 @@
 // TMEM is freed.
 #include <algorithm>
 #include "fp4.cuh"
+#include "fp4_tc.cuh"
 #include "launchers.h"
-#include "tc05.cuh"
 
 namespace g53 {
 namespace fp4 {
@@ -46,47 +46,6 @@ struct GemmCfg {
   static constexpr int kSmem = kStages * kStage + 1024;
   static constexpr uint32_t kBuf = BN == 256 ? 192 : 128;   // column of the second accumulator
 };
-
-// instruction descriptor of the 4-bit block-scaled kinds: A, B e2m1, K-major; scale type (0 e4m3, 1 E8M0); M; N; scale
-// data ids (which half of a 32-bit scale column the mma uses: 2X only)
-__device__ __forceinline__ uint32_t idesc4(int m, int n, bool ue8m0, uint32_t sf_id) {
-  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
-         ((uint32_t)(m >> 7) << 27) | (sf_id << 29);
-}
-
-template <bool NV>
-__device__ __forceinline__ void mma4(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t sfa, uint32_t sfb,
-                                     uint32_t acc) {
-  if constexpr (NV) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"(acc));
-  } else {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(sfa), "r"(sfb), "r"(acc));
-  }
-}
-
-// one scale atom (32 rows x 16 bytes) -> 4 TMEM columns, repeated in the four lane quadrants.  Descriptor: no swizzle,
-// 8-row groups 128 bytes apart
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
-  uint64_t d = (uint64_t)((smem >> 4) & 0x3FFF);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(128 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d));
-}
-
-__device__ __forceinline__ void gm_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(tc::saddr(dst)), "l"(src), "r"(bytes), "r"(tc::saddr(bar)) : "memory");
-}
-__device__ __forceinline__ void gm_expect(uint64_t* b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::saddr(b)), "r"(bytes) : "memory");
-}
 
 __device__ __forceinline__ void tile_mn(int t, int MT, int NT, int& m, int& n) {
   const int band = t / (kBandM * NT);
@@ -248,7 +207,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
   const uint32_t tmem = tmem_s;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t it = 0;
       bool ok = true;
       for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
@@ -263,14 +222,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
           }
           uint8_t* a = smem + s * C::kStage;
           uint8_t* sa = a + (1 + C::kNB) * kTileBytes;
-          gm_expect(&full[s], (uint32_t)(1 + nblk) * (kTileBytes + C::kSB));
+          bulk_expect(&full[s], (uint32_t)(1 + nblk) * (kTileBytes + C::kSB));
           const int64_t ta = (int64_t)mb * KT + kt;
-          gm_bulk(a, p.a_codes + ta * kTileBytes, kTileBytes, &full[s]);
-          gm_bulk(sa, p.a_scales + ta * C::kSB, C::kSB, &full[s]);
+          bulk_load(a, p.a_codes + ta * kTileBytes, kTileBytes, &full[s]);
+          bulk_load(sa, p.a_scales + ta * C::kSB, C::kSB, &full[s]);
           for (int b = 0; b < nblk; ++b) {
             const int64_t tb = (int64_t)(nt * C::kNB + b) * KT + kt;
-            gm_bulk(a + (1 + b) * kTileBytes, p.b_codes + tb * kTileBytes, kTileBytes, &full[s]);
-            gm_bulk(sa + (1 + b) * C::kSB, p.b_scales + tb * C::kSB, C::kSB, &full[s]);
+            bulk_load(a + (1 + b) * kTileBytes, p.b_codes + tb * kTileBytes, kTileBytes, &full[s]);
+            bulk_load(sa + (1 + b) * C::kSB, p.b_scales + tb * C::kSB, C::kSB, &full[s]);
           }
         }
       }
@@ -282,7 +241,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t it = 0, tl = 0;
       bool ok = true;
       for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++tl) {

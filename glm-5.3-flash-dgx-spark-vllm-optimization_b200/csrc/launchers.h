@@ -413,10 +413,21 @@ struct Fp4DequantArgs {
 };
 cudaError_t g53_fp4_dequant(const Fp4DequantArgs& p, cudaStream_t st);
 
-// y[M, N] (mode) = x[M, K] bf16 @ W4[N, K]^T, M <= 16 (fp4_gemv.cu).  GEMV_SWIGLU: W4 is a gate/up image (64 gate rows,
-// then their 64 up rows, per 128-row block), y [M, width] bf16
-struct Fp4GemvArgs {
-  const __nv_bfloat16* x; int64_t ldx; int xvec;
+// Expansion of M <= 32 bf16 rows into g53_fp4_terms() 4-bit rows each (fp4_skinny.cu): image rows terms * m + t
+int g53_fp4_terms();
+struct Fp4ExpandArgs {
+  const __nv_bfloat16* x; int64_t ldx;
+  int M, K, nv;
+  int vec;                             // 16-byte aligned rows
+  uint8_t* codes; uint8_t* scales;
+  float* factor;                       // [M] power of two of the row (nvfp4), 1 (mxfp4)
+};
+cudaError_t g53_fp4_expand(const Fp4ExpandArgs& p, cudaStream_t st);
+
+// y[M, N] (mode) = x[M, K] @ W4[N, K]^T for expanded rows, M <= 32 (fp4_skinny.cu).  GEMV_SWIGLU: W4 is a gate/up image
+// (64 gate rows, then their 64 up rows, per 128-row block), y [M, width] bf16
+struct Fp4SkinnyArgs {
+  const uint8_t* x_codes; const uint8_t* x_scales; const float* x_factor;
   const uint8_t* codes; const uint8_t* scales; const float* row_scale;
   int nv;
   void* y; int64_t ldy;
@@ -425,7 +436,7 @@ struct Fp4GemvArgs {
   int mode;
   float limit;
 };
-cudaError_t g53_fp4_gemv(const Fp4GemvArgs& p, cudaStream_t st);
+cudaError_t g53_fp4_skinny(const Fp4SkinnyArgs& p, cudaStream_t st);
 
 // y[M, N] (mode) = A4[M, K] @ W4[N, K]^T on the block-scaled tensor-core path (fp4_gemm.cu).  out_* (GEMV_SWIGLU): the
 // activations are written as a 4-bit image [M, width] with the row scale 2^h_exp (nvfp4)
@@ -445,5 +456,5 @@ cudaError_t g53_fp4_gemm(const Fp4GemmArgs& p, cudaStream_t st);
 // the current device's error word of the large-M kernels (bounded waits)
 cudaError_t g53_fp4_gemm_error_word(int** word);
 // first error code recorded on the current device by a bounded wait of these kernels (0: none); clears it
-cudaError_t g53_fp4_gemv_error(int* code);
+cudaError_t g53_fp4_skinny_error(int* code);
 cudaError_t g53_fp4_gemm_error(int* code);

@@ -69,6 +69,20 @@ def sums_tol(a, w):
     return 2 * a.shape[1] * 2.0 ** -23 * (a.abs() @ w.abs().t())
 
 
+def act_tol(x, w, fmt):
+    """Bound of what the 8-term expansion of 16-bit activations leaves out (x, w in 64 bits).  nvfp4: the block scale is
+    within 1/16 of a sixth of the maximum, and rounding leaves at most one scale: (17/96)^8 < 2^-19 of the block's
+    maximum; a block whose scale underflows e4m3 waits for a later term, whose row factor is smaller: 2^-31 of the row's
+    maximum.  mxfp4: the first scale is under a third of the maximum, each next one a quarter of the last: 4^-7 / 3 <
+    2^-15."""
+    blk = 16 if fmt == "nvfp4" else 32
+    amax = x.abs().view(x.shape[0], -1, blk).amax(-1)
+    wsum = w.abs().view(w.shape[0], -1, blk).sum(-1)
+    if fmt == "mxfp4":
+        return 2.0 ** -15 * amax @ wsum.t()
+    return (2.0 ** -19 * amax + 2.0 ** -31 * amax.amax(1, keepdim=True)) @ wsum.t()
+
+
 def half(dtype):
     return torch.finfo(dtype).eps / 2
 
@@ -149,8 +163,7 @@ def test_linear_few_rows(fmt, n, k, m):
     w4 = fp4.quantize4(w, fmt)
     wq = quant(w, fmt)
     ref = x.double() @ wq.t()
-    # f16 activations: off by at most 2^-39 of the row's largest
-    tol = sums_tol(x.double(), wq) + 2.0 ** -39 * x.double().abs().amax(1, keepdim=True) * wq.abs().sum(1)
+    tol = sums_tol(x.double(), wq) + act_tol(x.double(), wq, fmt)
     y = fp4.linear4(x, w4, torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32)
     assert ((y.double() - ref).abs() <= tol).all()
     yb = fp4.linear4(x, w4, torch.empty(m, n, dtype=BF, device="cuda"))
@@ -176,7 +189,7 @@ def test_linear_few_rows_magnitudes_and_views(fmt):
     for off in (0, 1, 8):
         x = big[0:22:2, off:off + k]
         ref = x.double() @ wq.t()
-        tol = sums_tol(x.double(), wq) + 2.0 ** -39 * x.double().abs().amax(1, keepdim=True) * wq.abs().sum(1)
+        tol = sums_tol(x.double(), wq) + act_tol(x.double(), wq, fmt)
         out = torch.full((13, 301), 5.0, dtype=F32, device="cuda")
         fp4.linear4(x, w4, out[1:12, 3:203], K.GEMV_F32)
         y = out[1:12, 3:203].double()
@@ -213,7 +226,7 @@ def test_linear_exact_activations_above_16_rows(fmt, m):
     x, w = acts(m, k, m), weight(n, k, 5)
     w4, wq = fp4.quantize4(w, fmt), quant(w, fmt)
     ref = x.double() @ wq.t()
-    tol = sums_tol(x.double(), wq) + 2.0 ** -39 * x.double().abs().amax(1, keepdim=True) * wq.abs().sum(1)
+    tol = sums_tol(x.double(), wq) + act_tol(x.double(), wq, fmt)
     y = fp4.linear4(x, w4, torch.zeros(m, n, dtype=F32, device="cuda"), K.GEMV_F32)
     assert ((y.double() - ref).abs() <= tol).all()
     y2 = fp4.linear4(x, w4, y.clone(), K.GEMV_F32_ACC)
@@ -221,7 +234,7 @@ def test_linear_exact_activations_above_16_rows(fmt, m):
     odd = acts(m, k + 1, m)[:, 1:]
     ref = odd.double() @ wq.t()
     y = fp4.linear4(odd, w4, torch.zeros(m, n, dtype=BF, device="cuda"))
-    tol = sums_tol(odd.double(), wq) + 2.0 ** -39 * odd.double().abs().amax(1, keepdim=True) * wq.abs().sum(1)
+    tol = sums_tol(odd.double(), wq) + act_tol(odd.double(), wq, fmt)
     assert ((y.double() - ref).abs() <= tol + half(BF) * (ref.abs() + tol)).all()
 
 
@@ -307,14 +320,12 @@ def test_mlp_exact_activations(fmt, m, k, width, n):
     xd = x.double()
     h = gated(xd, gq, uq, limit)
     # gate and up sums, then the activation (derivative at most 1.1 limit in either), exp and the division: 2^-20
-    far = 2.0 ** -39 * xd.abs().amax(1, keepdim=True)
-    eg = sums_tol(xd, gq) + far * gq.abs().sum(1)
-    eu = sums_tol(xd, uq) + far * uq.abs().sum(1)
+    eg = sums_tol(xd, gq) + act_tol(xd, gq, fmt)
+    eu = sums_tol(xd, uq) + act_tol(xd, uq, fmt)
     eh = 1.1 * limit * (eg + eu) + 2.0 ** -20 * h.abs()
     eh = eh + half(BF) * (h.abs() + eh)
     ref = h @ dq.t()
-    hmax = h.abs().amax(1, keepdim=True) * (1 + half(BF))
-    tol = eh @ dq.abs().t() + sums_tol(h, dq) * (1 + half(BF)) + 2.0 ** -39 * hmax * dq.abs().sum(1)
+    tol = eh @ dq.abs().t() + sums_tol(h.abs() + eh, dq) + act_tol(h.abs() + eh, dq, fmt)
     y = fp4.mlp4(x, mlp, torch.empty(m, n, dtype=F32, device="cuda"), limit)
     assert ((y.double() - ref).abs() <= tol).all()
     yb = fp4.mlp4(x, mlp, torch.empty(m, n, dtype=BF, device="cuda"), limit, K.GEMV_BF16)
