@@ -140,49 +140,44 @@ void check_xy(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int
               op, ": y must be [", num(x.size(0)), ", ", num(n), "], rows contiguous and apart");
 }
 
-// 4-bit expansion of some rows of x (scratch of one call)
-struct Expanded {
-  Tensor codes, scales, factor;
-  int M;
-};
-
-Expanded expand(const Tensor& x, int64_t m0, int64_t m, bool nv) {
-  const int64_t K = x.size(1), tiles = (m * g53_fp4_terms() + kTileRows - 1) / kTileRows * ((K + kTileK - 1) / kTileK);
-  const int64_t sb = kTileRows * (kTileK / (nv ? 16 : 32));
-  const Tensor buf = torch::empty({tiles * (kTileBytes + sb) + m * 4}, x.options().dtype(at::kByte));
-  Expanded e{buf.narrow(0, 0, tiles * kTileBytes), buf.narrow(0, tiles * kTileBytes, tiles * sb),
-             buf.narrow(0, tiles * (kTileBytes + sb), m * 4), (int)m};
-  Fp4ExpandArgs a{};
-  a.x = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()) + m0 * x.stride(0);
-  a.ldx = x.stride(0);
-  a.M = (int)m;
-  a.K = (int)K;
-  a.nv = nv;
-  a.vec = aligned16(a.x) && a.ldx % 8 == 0;
-  a.codes = e.codes.data_ptr<uint8_t>();
-  a.scales = e.scales.data_ptr<uint8_t>();
-  a.factor = reinterpret_cast<float*>(e.factor.data_ptr());
-  ok(g53_fp4_expand(a, stream()), "fp4_expand");
-  return e;
-}
-
 // all rows of x through the small-M kernel, kSkinnyRows at a time
 void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t width, int64_t mode, double limit) {
+  const int64_t K = w.k, sb = kTileRows * (kTileK / (w.nv ? 16 : 32));
   for (int64_t m0 = 0; m0 < x.size(0); m0 += kSkinnyRows) {
-    const Expanded e = expand(x, m0, std::min(kSkinnyRows, x.size(0) - m0), w.nv);
+    const int64_t m = std::min(kSkinnyRows, x.size(0) - m0);
+    const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()) + m0 * x.stride(0);
+    const int vec = aligned16(rows) && x.stride(0) % 8 == 0;
     Fp4SkinnyArgs a{};
-    a.x_codes = e.codes.data_ptr<uint8_t>();
-    a.x_scales = e.scales.data_ptr<uint8_t>();
-    a.x_factor = reinterpret_cast<const float*>(e.factor.data_ptr());
+    Tensor buf;
+    if (g53_fp4_expand_inline((int)m, n, (int)K, w.nv)) {
+      a.x = rows;
+      a.ldx = x.stride(0);
+      a.xvec = vec;
+    } else {
+      const int64_t tiles = (m * g53_fp4_terms() + kTileRows - 1) / kTileRows * ((K + kTileK - 1) / kTileK);
+      buf = torch::empty({tiles * (kTileBytes + sb) + m * 4}, x.options().dtype(at::kByte));
+      uint8_t* b = buf.data_ptr<uint8_t>();
+      Fp4ExpandArgs e{};
+      e.x = rows;
+      e.ldx = x.stride(0);
+      e.M = (int)m;
+      e.K = (int)K;
+      e.nv = w.nv;
+      e.vec = vec;
+      a.x_codes = e.codes = b;
+      a.x_scales = e.scales = b + tiles * kTileBytes;
+      a.x_factor = e.factor = reinterpret_cast<float*>(b + tiles * (kTileBytes + sb));
+      ok(g53_fp4_expand(e, stream()), "fp4_expand");
+    }
     a.codes = w.c();
     a.scales = w.s();
     a.row_scale = w.r();
     a.nv = w.nv;
     a.y = reinterpret_cast<uint8_t*>(y.data_ptr()) + m0 * y.stride(0) * y.element_size();
     a.ldy = y.stride(0);
-    a.M = e.M;
+    a.M = (int)m;
     a.N = (int)n;
-    a.K = (int)w.k;
+    a.K = (int)K;
     a.width = (int)width;
     a.mode = (int)mode;
     a.limit = (float)limit;

@@ -3,21 +3,25 @@
 // A decode projection reads every weight byte once, so HBM is the floor: 9/16 (17/32) byte per weight.  Widening the
 // weights to f16 operands on the CUDA cores cannot keep up with that (built first: 390 instructions per warp and 32 x 128
 // weights, 2.7 TB/s), so the codes go to the block-scaled tensor cores as they are, as the 128-row operand of
-// tcgen05.mma, and the activations are brought to 4 bits without losing them: each row is expanded into kTerms = 8 rows
-//     x = sum_t Q(r_t),   r_0 = x,   r_{t+1} = r_t - Q(r_t)
-// of the weights' own format, which become 8 of the mma's N columns.  The fp32 columns of a row are summed in the epilogue.
-// Every term leaves at most 0.177 (nvfp4) or 1/4 (mxfp4, after the first) of what was there, block by block, so the sum
-// of 8 is within 2^-19 (nvfp4) or 2^-15 (mxfp4) of a block's largest magnitude in the worst case; on normal activations
-// the residue is 4e-10 of the row's norm, or zero: an element of bf16's 8 bits is used up after 2 bits a term.  The tensor
-// core has the time: N = 64 (8 rows) costs 128 clocks per 128 x 256 tile of weights, HBM delivers one in 790 per SM.
+// tcgen05.mma, and the activations are brought to 4 bits without losing them: a block of x with largest magnitude in
+// [2^e, 2^(e+1)) is written as integers X = round(x 2^(21-e)), |X| < 2^22, and X in eight balanced base-8 digits,
+//     x = sum_t d_t 2^(e-3t),   d_t in -4..3, t = 0..7,
+// all of which are e2m1 values.  Term t of a row is a 4-bit row with the block scales 2^(e-3t); the eight of them are 8 of
+// the mma's N columns, and the epilogue sums the eight fp32 columns.  What is lost is at most 2^-22 of the block's largest
+// magnitude; a bf16 element within 2^-14 of it loses nothing.  The tensor core has the time: N = 64 (8 rows) costs about
+// 290 clocks per 128 x 256 tile of weights, HBM delivers one in 790 per SM.
 //
-// fp4_expand writes the expansion as a tile image (fp4.cuh), rows 8 m + t.  nvfp4: one power of two per row of x brings
-// the block scales into e4m3's range, term t uses 2^-kOff[t] of it; the epilogue puts both back.
+// nvfp4's e4m3 scales hold 2^(e-3t) over a power of two of the row and of the term, which the epilogue puts back; they
+// reach from 2^8 down to 2^-9, so a block more than 2^17 below the row's largest shares the scale of one at 2^-17 (off by
+// at most 2^-39 of the row's largest).
+//
+// The expansion is formed by each CTA for its own slice of K, in shared memory, when that is little work (INLINE); else
+// fp4_expand writes it once as a tile image (fp4.cuh), rows 8 m + t, and it is fetched tile by tile beside the weights.
 //
 // fp4_skinny: a CTA takes a 128-row block of W and a slice of its K tiles; a cluster of CL CTAs shares a block, and
-// clusters walk the blocks.  Warp 0 streams tiles of both operands into a ring (contiguous cp.async.bulk), warp 1 copies
-// the scales to TMEM and issues the mma, warps 2-5 read the sums (a thread holds one weight row), send them to the rank of
-// the cluster that owns the row (distributed shared memory, one arrival per sender) and finish the rows they own, adding
+// clusters walk the blocks.  Warp 0 streams tiles into a ring (contiguous cp.async.bulk), warp 1 copies the scales to TMEM
+// and issues the mma, warps 2-5 (form the expansion,) read the sums (a thread holds one weight row), send them to the rank
+// of the cluster that owns the row (distributed shared memory, one arrival per sender) and finish the rows they own, adding
 // in rank order: the result does not depend on timing.  Two receive buffers alternate: a rank can only send block b + 2
 // after it received every rank's b + 1, which each sent after it had finished reading b.
 //
@@ -25,6 +29,7 @@
 // Waits are bounded; one that runs out sets the error word and the CTA goes on without waiting, so every barrier is
 // still reached, copies and mma in flight are waited for (bounded) and the TMEM is freed.
 #include <algorithm>
+#include <atomic>
 #include <cooperative_groups.h>
 #include "fp4.cuh"
 #include "fp4_tc.cuh"
@@ -38,12 +43,107 @@ namespace fp4 {
 __device__ int g_skinny_err = 0;
 
 constexpr int kTerms = 8;
-__host__ __device__ constexpr int term_off(int t) { return (5 * t) / 2; }     // 0 2 5 7 10 12 15 17
-constexpr int kSkThreads = 192;
+constexpr int kEpi = 4;                               // warps of the expansion and the epilogue
+constexpr int kSkThreads = 64 + kEpi * 32;
 constexpr int kErrSk = 0x6b40;
 
 // ------------------------------------------------------------------------------------------------------ expansion
-// CTA: 128 blocks of 16 of one row (a thread each); nvfp4 reads the whole row for its maximum first.
+// 16 elements (bf16 pairs) of a block with exponent e -> word t of each term: 8 bytes of codes.  X' = X + sum_t 4 * 8^t has
+// the digits d_t + 4 as its octal digits; a byte permutation looks up the codes of 4 digits at a time, even elements in
+// the low and odd ones in the high nibble.
+template <typename F>
+__device__ __forceinline__ void expand16(const uint32_t (&w)[8], int e, F&& emit) {
+  const float s = pow2i(21 - e);
+  uint32_t x[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // 1.5 * 2^23 + X: X in the low bits of the float
+    constexpr uint32_t kShift = 044444444u - 0x4b400000u;
+    x[2 * i] = __float_as_uint(fmaf(__uint_as_float(w[i] << 16), s, 12582912.f)) + kShift;
+    x[2 * i + 1] = __float_as_uint(fmaf(__uint_as_float(w[i] & 0xffff0000u), s, 12582912.f)) + kShift;
+  }
+#pragma unroll
+  for (int t = 0; t < kTerms; ++t) {
+    const int sh = 3 * (kTerms - 1 - t);
+    uint32_t code[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t lo = 0, hi = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = x[8 * h + 2 * i], b = x[8 * h + 2 * i + 1];
+        lo |= (sh >= 4 * i ? a >> (sh - 4 * i) : a << (4 * i - sh)) & (7u << (4 * i));
+        hi |= (sh >= 4 * i ? b >> (sh - 4 * i) : b << (4 * i - sh)) & (7u << (4 * i));
+      }
+      // codes of the digits -4 -3 -2 -1 0 1 2 3: 14 13 12 10 0 2 4 5
+      code[h] = __byte_perm(0x0a0c0d0eu, 0x05040200u, lo) | __byte_perm(0xa0c0d0e0u, 0x50402000u, hi);
+    }
+    emit(t, make_uint2(code[0], code[1]));
+  }
+}
+
+__device__ __forceinline__ uint32_t amax_bits16(const uint32_t (&w)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
+  return m;
+}
+__device__ __forceinline__ void load16(const uint16_t* x, bool vec, uint32_t (&w)[8]) {
+  if (vec) {
+    const uint4 a = *reinterpret_cast<const uint4*>(x), c = *reinterpret_cast<const uint4*>(x + 8);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = (uint32_t)x[2 * i] | ((uint32_t)x[2 * i + 1] << 16);
+  }
+}
+__device__ __forceinline__ int exponent(uint32_t bits) { return (int)(bits >> 23) - 127; }
+// nvfp4: exponent of the row, low enough rows share one (2^(21-e) stays in range)
+__device__ __forceinline__ int row_exponent(uint32_t amax) { return max(exponent(amax), -85); }
+__device__ __forceinline__ float row_factor(uint32_t amax) {
+  return amax >= kInfBits ? __uint_as_float(0x7fc00000u) : pow2i(max(row_exponent(amax) - 8, -126));
+}
+
+// block of 16 -> exponent and scale byte(s).  nvfp4: one byte for all terms (the term's 2^-3t is put back later); mxfp4:
+// byte of term 0, term t is 3t lower
+template <bool NV>
+__device__ __forceinline__ int block_exponent(uint32_t amax, int row_e, uint32_t& byte) {
+  if constexpr (NV) {
+    const int e = max(min(exponent(amax), row_e), row_e - 17);
+    const int n = e - row_e + 8;                      // 8 .. -9
+    byte = n >= -6 ? (uint32_t)(n + 7) << 3 : 1u << (n + 9);
+    return e;
+  } else {
+    const int e = max(exponent(amax), -105);
+    byte = amax >= kInfBits ? 255u : (uint32_t)(e + 127);
+    return min(e, 127);
+  }
+}
+template <bool NV>
+__device__ __forceinline__ uint32_t term_scales(uint32_t s4, int t) {
+  if constexpr (NV) return s4;
+  // four E8M0 bytes, each 3t lower unless NaN (byte-wise: no borrow, every byte is >= 22 or 0 for padding)
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = (s4 >> (8 * i)) & 0xffu;
+    r |= (b == 255u ? 255u : b > 3u * t ? b - 3u * t : 0u) << (8 * i);
+  }
+  return r;
+}
+// scale bytes of four neighbouring columns in one word (valid in the first of their lanes)
+template <bool NV>
+__device__ __forceinline__ uint32_t gather_scales(uint32_t sc) {
+  constexpr int kStep = NV ? 1 : 2;
+  uint32_t s4 = sc;
+  s4 |= __shfl_down_sync(0xffffffffu, sc, kStep) << 8;
+  s4 |= __shfl_down_sync(0xffffffffu, sc, 2 * kStep) << 16;
+  s4 |= __shfl_down_sync(0xffffffffu, sc, 3 * kStep) << 24;
+  return s4;
+}
+
+// CTA: 128 blocks of 16 of one row (a thread each); nvfp4 reads the whole row for its maximum first
 template <bool NV>
 __global__ void __launch_bounds__(128) fp4_expand_kernel(Fp4ExpandArgs p) {
   __shared__ uint32_t red[4];
@@ -54,110 +154,47 @@ __global__ void __launch_bounds__(128) fp4_expand_kernel(Fp4ExpandArgs p) {
   pdl_trigger();
   pdl_wait();
   uint32_t w[8];
-  auto load = [&](int blk) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 0u;
-    if (blk < nk) {
-      if (p.vec) {
-        const uint4 a = *reinterpret_cast<const uint4*>(x + (int64_t)blk * 16);
-        const uint4 c = *reinterpret_cast<const uint4*>(x + (int64_t)blk * 16 + 8);
-        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          w[i] = (uint32_t)x[(int64_t)blk * 16 + 2 * i] | ((uint32_t)x[(int64_t)blk * 16 + 2 * i + 1] << 16);
-      }
-    }
-  };
-  float scale = 1.f;
+  int row_e = 0;
   if constexpr (NV) {
     uint32_t am = 0;
     for (int blk = threadIdx.x; blk < nk; blk += 128) {
-      load(blk);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) am = max(am, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
+      load16(x + (int64_t)blk * 16, p.vec, w);
+      am = max(am, amax_bits16(w));
     }
     am = __reduce_max_sync(0xffffffffu, am);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = am;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) am = max(am, red[i]);
-    const int k = am >= kInfBits ? 0 : nv_row_exp(am);
-    scale = pow2i(-k);
-    if (b == 0) p.factor[m] = am >= kInfBits ? __uint_as_float(0x7fc00000u) : pow2i(k);
+    row_e = row_exponent(am);
+    if (b == 0) p.factor[m] = row_factor(am);
   } else if (b == 0) {
     p.factor[m] = 1.f;
   }
-  load(b);
-  float r[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    r[2 * i] = __uint_as_float(w[i] << 16) * scale;
-    r[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * scale;
-  }
+  for (int i = 0; i < 8; ++i) w[i] = 0u;
+  if (b < nk) load16(x + (int64_t)b * 16, p.vec, w);
+  uint32_t am = amax_bits16(w), sc;
+  if (!NV) am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
+  const int e = block_exponent<NV>(am, row_e, sc);
+  const uint32_t s4 = gather_scales<NV>(b < nk ? sc : 0u);
   const int kt = b >> 4, kb = b & 15;
-#pragma unroll
-  for (int t = 0; t < kTerms; ++t) {
-    const int row = m * kTerms + t;                  // row of the expansion, < 256
-    const int rr = row % kTileRows;
-    const int64_t tile = (int64_t)(row / kTileRows) * KT + kt;
-    if (NV && t > 0) {
-      const float up = pow2i(term_off(t) - term_off(t - 1));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) r[i] *= up;
-    }
-    uint32_t am = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) am = max(am, __float_as_uint(r[i]) & 0x7fffffffu);
-    uint32_t sc;
-    float s, inv;
-    if constexpr (NV) {
-      const __nv_fp8_e4m3 q(__uint_as_float(am) * 0.16666667f);      // any scale near a sixth does here
-      sc = am >= kInfBits ? 0x7fu : q.__x;
-      s = e4m3_to_f32(sc);
-      inv = s > 0.f ? __frcp_rn(s) : 0.f;
-    } else {
-      am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
-      sc = mx_scale(am);
-      s = e8m0_to_f32(sc);
-      inv = sc == 255u ? 0.f : pow2i(127 - (int)sc);
-    }
-    uint32_t code[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = r[8 * h + i] * inv;
-      code[h] = f32x8_to_e2m1(f);
-      uint32_t o[4];
-      e2m1x8_to_f16(code[h], o);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&o[i]));
-        r[8 * h + 2 * i] = fmaf(-v.x, s, r[8 * h + 2 * i]);
-        r[8 * h + 2 * i + 1] = fmaf(-v.y, s, r[8 * h + 2 * i + 1]);
-      }
-    }
-    if (b >= nk) sc = 0u;
-    constexpr int kStep = NV ? 1 : 2;
-    uint32_t s4 = sc;
-    s4 |= __shfl_down_sync(0xffffffffu, sc, kStep) << 8;
-    s4 |= __shfl_down_sync(0xffffffffu, sc, 2 * kStep) << 16;
-    s4 |= __shfl_down_sync(0xffffffffu, sc, 3 * kStep) << 24;
-    if (b < nb) {
-      *reinterpret_cast<uint2*>(p.codes + tile * kTileBytes + chunk_off(rr, kb >> 1) + (kb & 1) * 8) =
-          make_uint2(code[0], code[1]);
+  if (b < nb)
+    expand16(w, e, [&](int t, uint2 code) {
+      const int row = m * kTerms + t, rr = row % kTileRows;
+      const int64_t tile = (int64_t)(row / kTileRows) * KT + kt;
+      *reinterpret_cast<uint2*>(p.codes + tile * kTileBytes + chunk_off(rr, kb >> 1) + (kb & 1) * 8) = code;
+      constexpr int kStep = NV ? 1 : 2;
       if ((kb & (4 * kStep - 1)) == 0)
-        *reinterpret_cast<uint32_t*>(p.scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, kb / kStep)) = s4;
-    }
-  }
+        *reinterpret_cast<uint32_t*>(p.scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, kb / kStep)) =
+            term_scales<NV>(s4, t);
+    });
 }
 
 // -------------------------------------------------------------------------------------------------------- product
-// per: K tiles of a slice; stages: ring depth; clusters: persistent clusters; ncol: mma N
+// per: K tiles of a slice; stages: ring depth; clusters: persistent clusters; ncol: mma N; xbytes: resident expansion
 struct SkPlan {
-  int blocks, KT, per, stages, clusters, CL, ncol, stage_bytes, mp;
+  int blocks, KT, per, stages, clusters, CL, ncol, stage_bytes, xbytes;
 };
 
 __device__ __forceinline__ bool sk_wait(uint64_t* b, uint32_t ph, volatile int* stop, bool drain = false) {
@@ -192,9 +229,11 @@ __device__ __forceinline__ void sk_sync() { asm volatile("bar.sync 1, 128;" ::: 
 __device__ __forceinline__ void sk_prefetch(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // WIDE: mma N up to 256 (17..32 rows), one CTA per SM; otherwise N <= 128 and two CTAs per SM
-template <bool NV, bool WIDE>
+template <bool NV, bool WIDE, bool INLINE>
 __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp4SkinnyArgs p, SkPlan pl) {
   constexpr int kSB = Fmt<NV>::kScaleBytes;
   constexpr int kAtoms = kSB / 512;
@@ -202,12 +241,14 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
   constexpr uint32_t kCols = WIDE ? 512 : 256;        // TMEM columns: sums, scales of W, scales of X
   constexpr uint32_t kSfW = WIDE ? 256 : 128, kSfX = kSfW + 16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[8], empty[8], recv_bar[2], tfull, tempty, drain;
-  __shared__ uint32_t tmem_s;
+  __shared__ __align__(8) uint64_t full[8], empty[8], recv_bar[2], tfull, tempty, xready, drain;
+  __shared__ uint32_t tmem_s, xmax[32];
+  __shared__ float xfac[32];
   __shared__ int stop_s;
   volatile int* stop = &stop_s;
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* recv = reinterpret_cast<float*>(ring + pl.stages * pl.stage_bytes);   // [2][CL][mp][2][j_per]
+  uint8_t* xs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = xs + (INLINE ? pl.xbytes : 0);
+  float* recv = reinterpret_cast<float*>(ring + pl.stages * pl.stage_bytes);   // [2][CL][M][2][j_per]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int CL = pl.CL;
@@ -216,9 +257,11 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
   // rows of a block that this rank finishes: pairs (j, j + 64), j in [j_lo, j_lo + rows)
   const int j_per = (64 + CL - 1) / CL;
   const int j_lo = min(64, rank * j_per), rows = min(64, j_lo + j_per) - j_lo;
-  const int xrows = pl.ncol;                          // rows of the expansion that are fetched
+  const int xrows = pl.ncol;                          // rows of the expansion
   const int xb0 = min(xrows, 128) * 128, xb1 = WIDE ? max(0, xrows - 128) * 128 : 0;
-  const int off_x = kTileBytes, off_sw = off_x + xrows * 128, off_sx = off_sw + kSB;
+  const int xtile = xrows * 128;                      // code bytes of the expansion per K tile
+  // a stage: codes of W, (codes of X,) scales of W, (scales of X)
+  const int off_x = kTileBytes, off_sw = off_x + (INLINE ? 0 : xtile), off_sx = off_sw + kSB;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < pl.stages; ++s) {
@@ -228,15 +271,18 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
     tc::bar_init(&recv_bar[0], CL > 1 ? CL - 1 : 1);
     tc::bar_init(&recv_bar[1], CL > 1 ? CL - 1 : 1);
     tc::bar_init(&tfull, 1);
-    tc::bar_init(&tempty, 4);
+    tc::bar_init(&tempty, kEpi);
+    tc::bar_init(&xready, kEpi);
     tc::bar_init(&drain, 1);
     stop_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x >= 64 && threadIdx.x < 96) xmax[threadIdx.x - 64] = 0;
   if (warp == 1) tc::tmem_alloc(&tmem_s, kCols);
   tc::fence_before();
-  if (CL > 1) cg::this_cluster().sync();
-  else __syncthreads();
+  __syncthreads();
+  // the peers' barriers are first touched by the epilogue, which waits there
+  if (CL > 1) cluster_arrive();
   tc::fence_after();
   const uint32_t tmem = tmem_s;
   pdl_trigger();
@@ -258,15 +304,17 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
           const uint32_t round = it / pl.stages;
           if (round > 0 && !sk_wait(&empty[s], (round - 1) & 1, stop)) { ok = false; break; }
           uint8_t* dst = ring + s * pl.stage_bytes;
-          bulk_expect(&full[s], (uint32_t)(kTileBytes + kSB + xb0 + kSB + (WIDE && xb1 ? xb1 + kSB : 0)));
+          bulk_expect(&full[s], (uint32_t)(kTileBytes + kSB + (INLINE ? 0 : xb0 + kSB + (WIDE && xb1 ? xb1 + kSB : 0))));
           const int64_t tw = (int64_t)nb * pl.KT + t;
           bulk_load_hint(dst, p.codes + tw * kTileBytes, kTileBytes, &full[s], pol);
           bulk_load_hint(dst + off_sw, p.scales + tw * kSB, kSB, &full[s], pol);
-          bulk_load(dst + off_x, p.x_codes + (int64_t)t * kTileBytes, xb0, &full[s]);
-          bulk_load(dst + off_sx, p.x_scales + (int64_t)t * kSB, kSB, &full[s]);
-          if (WIDE && xb1) {
-            bulk_load(dst + off_x + kTileBytes, p.x_codes + (int64_t)(pl.KT + t) * kTileBytes, xb1, &full[s]);
-            bulk_load(dst + off_sx + kSB, p.x_scales + (int64_t)(pl.KT + t) * kSB, kSB, &full[s]);
+          if constexpr (!INLINE) {
+            bulk_load(dst + off_x, p.x_codes + (int64_t)t * kTileBytes, xb0, &full[s]);
+            bulk_load(dst + off_sx, p.x_scales + (int64_t)t * kSB, kSB, &full[s]);
+            if (WIDE && xb1) {
+              bulk_load(dst + off_x + kTileBytes, p.x_codes + (int64_t)(pl.KT + t) * kTileBytes, xb1, &full[s]);
+              bulk_load(dst + off_sx + kSB, p.x_scales + (int64_t)(pl.KT + t) * kSB, kSB, &full[s]);
+            }
           }
         }
       }
@@ -277,11 +325,15 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       }
     }
     __syncwarp();
+    if (CL > 1) {
+      cluster_wait();
+      cluster_arrive();
+    }
   } else if (warp == 1) {
     if (elect_one()) {
       const int ksteps = (p.K + 63) / 64;
       uint32_t it = 0, blk = 0;
-      bool ok = true;
+      bool ok = !INLINE || sk_wait(&xready, 0, stop);
       for (int nb = cid; nb < pl.blocks && ok; nb += pl.clusters, ++blk) {
         if (blk > 0 && !sk_wait(&tempty, (blk - 1) & 1, stop)) break;
         tc::fence_after();
@@ -290,12 +342,14 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
           if (!sk_wait(&full[s], (it / pl.stages) & 1, stop)) { ok = false; break; }
           tc::fence_after();
           const uint32_t a = tc::saddr(ring + s * pl.stage_bytes);
+          const uint32_t xc = INLINE ? tc::saddr(xs + (t - t_lo) * xtile) : a + off_x;
+          const uint32_t xsc = INLINE ? tc::saddr(xs + pl.per * xtile + (t - t_lo) * kSB) : a + off_sx;
 #pragma unroll
           for (int at = 0; at < kAtoms; ++at) {
             copy_scales(tmem + kSfW + at * 4, a + off_sw + at * 512);
 #pragma unroll
             for (int xb = 0; xb < kXB; ++xb)
-              copy_scales(tmem + kSfX + at * (4 * kXB) + xb * 4, a + off_sx + xb * kSB + at * 512);
+              copy_scales(tmem + kSfX + at * (4 * kXB) + xb * 4, xsc + xb * kSB + at * 512);
           }
           const int n = min(4, ksteps - t * 4);
 #pragma unroll
@@ -303,9 +357,8 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
             if (k >= n) break;
             const int at = NV ? k : k >> 1;
             const uint32_t sf = NV ? 0u : (uint32_t)(k & 1) * 2;
-            mma4<NV>(tmem, tc::desc_sw128(a + k * 32), tc::desc_sw128(a + off_x + k * 32),
-                     idesc4(128, pl.ncol, !NV, sf), tmem + kSfW + at * 4, tmem + kSfX + at * (4 * kXB),
-                     (t > t_lo || k > 0) ? 1u : 0u);
+            mma4<NV>(tmem, tc::desc_sw128(a + k * 32), tc::desc_sw128(xc + k * 32), idesc4(128, pl.ncol, !NV, sf),
+                     tmem + kSfW + at * 4, tmem + kSfX + at * (4 * kXB), (t > t_lo || k > 0) ? 1u : 0u);
           }
           tc::commit(&empty[s]);
         }
@@ -317,16 +370,71 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       }
     }
     __syncwarp();
+    if (CL > 1) {
+      cluster_wait();
+      cluster_arrive();
+    }
   } else {
-    const int quad = warp & 3, et = threadIdx.x - 64;
+    const int quad = warp & 3, et = threadIdx.x - 64, part = (warp - 2) >> 2;
     const int r = quad * 32 + lane;                   // row of the block
     const int j = r & 63, half = r >> 6;
     const int owner = j / j_per, jl = j - owner * j_per;
-    const int buf_floats = CL * pl.mp * 2 * j_per;
+    const int buf_floats = CL * p.M * 2 * j_per;
+    // finishing: this thread's row pair and its group's first (token, half)
+    const int groups = kEpi * 32 / rows;
+    const int f_row = et % rows, f_grp = et / rows;   // f_grp >= groups: no part in it
+    const bool swi = p.mode == GEMV_SWIGLU;
     pdl_wait();
+    if constexpr (INLINE) {
+      // a thread per block of 16 of the slice (the plan sees to it that there are no more than threads)
+      const int nblk = (t_hi - t_lo) * 16, nk = p.K / 16 - t_lo * 16;       // blocks in the slice; those that exist
+      const bool in = et < p.M * nblk;
+      const int m = in ? et / nblk : 0, b = et - m * nblk;
+      uint32_t w[8] = {};
+      if (in && b < nk)
+        load16(reinterpret_cast<const uint16_t*>(p.x) + (int64_t)m * p.ldx + (int64_t)t_lo * kTileK + b * 16, p.xvec, w);
+      uint32_t am = amax_bits16(w), sc;
+      if constexpr (NV) {
+        // the 16 lanes of a half warp belong to one row
+        const uint32_t hm = __reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, am);
+        if (in && (lane & 15) == 0) atomicMax(&xmax[m], hm);
+        sk_sync();
+        if (et < p.M) xfac[et] = row_factor(xmax[et]);
+      } else {
+        am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      }
+      const int e = block_exponent<NV>(am, NV ? row_exponent(xmax[m]) : 0, sc);
+      const uint32_t s4 = gather_scales<NV>(b < nk ? sc : 0u);
+      if (in) {
+        const int kb = b & 15;
+        uint8_t* xc = xs + (b >> 4) * xtile;
+        uint8_t* xsc = xs + pl.per * xtile + (b >> 4) * kSB;
+        expand16(w, e, [&](int t, uint2 code) {
+          const int row = m * kTerms + t;
+          *reinterpret_cast<uint2*>(xc + chunk_off(row, kb >> 1) + (kb & 1) * 8) = code;
+          constexpr int kStep = NV ? 1 : 2;
+          if ((kb & (4 * kStep - 1)) == 0)
+            *reinterpret_cast<uint32_t*>(xsc + scale_off(row, kb / kStep)) = term_scales<NV>(s4, t);
+        });
+      }
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::bar_arrive(&xready);
+    } else {
+      if (NV && et < p.M) xfac[et] = p.x_factor[et];
+    }
+    if (CL > 1) cluster_wait();                       // every CTA of the cluster has its barriers
+    sk_sync();
     uint32_t blk = 0;
     bool dead = false;
     for (int nb = cid; nb < pl.blocks; nb += pl.clusters, ++blk) {
+      // scales of the rows this thread will finish: loaded under the main loop
+      float rs0 = 1.f, rs1 = 1.f;
+      if (NV && f_grp < groups) {
+        const int n = nb * 128 + j_lo + f_row;
+        if (n < p.N) rs0 = __ldg(p.row_scale + n);
+        if (n + 64 < p.N) rs1 = __ldg(p.row_scale + n + 64);
+      }
       if (!dead) {
         int ok = 0;
         if (lane == 0) ok = sk_wait(&tfull, blk & 1, stop) ? 1 : 0;
@@ -334,11 +442,11 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       }
       float* rb = recv + (blk & 1) * buf_floats;
       // this rank's sums of row r, token tok -> [rank][tok][half][jl] of the owner
-      float* dst = rb + ((int64_t)rank * pl.mp * 2 + half) * j_per + jl;
+      float* dst = rb + ((int64_t)rank * p.M * 2 + half) * j_per + jl;
       if (CL > 1 && owner != rank) dst = cg::this_cluster().map_shared_rank(dst, owner);
       if (!dead) {
         tc::fence_after();
-        for (int m0 = 0; m0 < p.M; m0 += 4) {
+        for (int m0 = part * 4; m0 < p.M; m0 += kEpi) {
           float v[32];
           tc::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + m0 * kTerms, v);
 #pragma unroll
@@ -347,8 +455,8 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
             float sum = 0.f;
 #pragma unroll
             for (int t = kTerms - 1; t >= 0; --t)     // small terms first
-              sum = NV ? fmaf(v[i * kTerms + t], 1.f / (float)(1 << term_off(t)), sum) : sum + v[i * kTerms + t];
-            dst[(int64_t)(m0 + i) * 2 * j_per] = NV ? sum * p.x_factor[m0 + i] : sum;
+              sum = NV ? fmaf(v[i * kTerms + t], 1.f / (float)(1 << (3 * t)), sum) : sum + v[i * kTerms + t];
+            dst[(m0 + i) * 2 * j_per] = NV ? sum * xfac[m0 + i] : sum;
           }
         }
         tc::fence_before();
@@ -372,102 +480,160 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
         }
       }
       // ---- finish rows j_lo.. and + 64: consecutive threads on consecutive rows
-      const bool swi = p.mode == GEMV_SWIGLU;
-      const int halves = swi ? 1 : 2;
-      for (int e = et; e < rows * p.M * halves; e += 128) {
-        const int q = e / rows, row = e - q * rows;
-        const int tok = swi ? q : q >> 1, hf = swi ? 0 : q & 1;
-        float v = 0.f, u = 0.f;
-        for (int c = 0; c < CL; ++c) {
-          const float* src = rb + ((c * pl.mp + tok) * 2 + hf) * j_per + row;
-          v += src[0];
-          if (swi) u += src[j_per];
-        }
-        const int n = nb * 128 + j_lo + row + hf * 64;
-        if (swi) {
-          const int col = nb * 64 + j_lo + row;
-          if (col >= p.width) continue;
-          if (NV) {
-            v *= p.row_scale[n];
-            u *= p.row_scale[n + 64];
+      if (f_grp < groups) {
+        const int halves = swi ? 1 : 2;
+        for (int q = f_grp; q < p.M * halves; q += groups) {
+          const int tok = swi ? q : q >> 1, hf = swi ? 0 : q & 1;
+          float v = 0.f, u = 0.f;
+          for (int c = 0; c < CL; ++c) {
+            const float* src = rb + ((c * p.M + tok) * 2 + hf) * j_per + f_row;
+            v += src[0];
+            if (swi) u += src[j_per];
           }
-          // written so that a NaN stays one
-          v = v > p.limit ? p.limit : v;
-          u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
-          reinterpret_cast<__nv_bfloat16*>(p.y)[(int64_t)tok * p.ldy + col] = f2bf(siluf_(v) * u);
-        } else {
-          if (n >= p.N) continue;
-          if (NV) v *= p.row_scale[n];
-          const int64_t off = (int64_t)tok * p.ldy + n;
-          if (p.mode == GEMV_BF16) {
-            reinterpret_cast<__nv_bfloat16*>(p.y)[off] = f2bf(v);
+          if (swi) {
+            const int col = nb * 64 + j_lo + f_row;
+            if (col >= p.width) continue;
+            v *= rs0;
+            u *= rs1;
+            // written so that a NaN stays one
+            v = v > p.limit ? p.limit : v;
+            u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
+            reinterpret_cast<__nv_bfloat16*>(p.y)[(int64_t)tok * p.ldy + col] = f2bf(siluf_(v) * u);
           } else {
-            float* y = reinterpret_cast<float*>(p.y) + off;
-            *y = p.mode == GEMV_F32_ACC ? *y + v : v;
+            const int n = nb * 128 + j_lo + f_row + hf * 64;
+            if (n >= p.N) continue;
+            v *= hf ? rs1 : rs0;
+            const int64_t off = (int64_t)tok * p.ldy + n;
+            if (p.mode == GEMV_BF16) {
+              reinterpret_cast<__nv_bfloat16*>(p.y)[off] = f2bf(v);
+            } else {
+              float* y = reinterpret_cast<float*>(p.y) + off;
+              *y = p.mode == GEMV_F32_ACC ? *y + v : v;
+            }
           }
         }
       }
     }
+    __syncwarp();
+    if (CL > 1) cluster_arrive();
   }
   tc::fence_before();
   // no CTA leaves while another of its cluster may still write to it
-  if (CL > 1) cg::this_cluster().sync();
-  else __syncthreads();
+  if (CL > 1) cluster_wait();
+  __syncthreads();
   if (warp == 1) {
     tc::fence_after();
     tc::tmem_free(tmem, kCols);
   }
 }
 
-// Shape of the launch.  CL, the CTAs that share a row block, is the one that needs the fewest tile steps on the busiest
-// CTA (a block costs about one more step: its reduction and stores); ties go to the smaller, which sends less.
-template <bool NV, bool WIDE>
-static SkPlan sk_plan(int N, int K, int M, int sms) {
-  SkPlan b{};
-  b.blocks = (N + 127) / 128;
+constexpr int kMaxDev = 64;
+
+static int sk_recv_bytes(int CL, int M) { return 2 * CL * M * 2 * ((64 + CL - 1) / CL) * 4; }
+static int sk_budget(bool wide) { return (wide ? 225 : 111) * 1024; }
+
+// Stands in for the product in the question below: the runtime answers one CTA per SM for any kernel that uses TMEM
+template <bool WIDE>
+__global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) sk_shape_kernel() {}
+
+// clusters of CL CTAs that run at once on the current device (one or two CTAs per SM); asked once per device.  Not CTAs / CL:
+// a cluster stays inside a GPC (148 SMs: 296 CTAs alone, 93 clusters of 3, 33 of 8), and a cluster that has to wait for
+// another doubles the time.
+template <bool WIDE>
+static cudaError_t sk_active(int dev, int CL, int* out) {
+  static std::atomic<int> known[kMaxDev][9];
+  if (dev < kMaxDev && (*out = known[dev][CL].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  auto kern = sk_shape_kernel<WIDE>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sk_budget(WIDE));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(CL);
+  cfg.blockDim = dim3(kSkThreads);
+  cfg.dynamicSmemBytes = sk_budget(WIDE);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CL;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(out, kern, &cfg);
+  if (e != cudaSuccess) return e;
+  *out = std::max(*out, 1);
+  if (dev < kMaxDev) known[dev][CL].store(*out, std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
+// the dynamic shared memory limit of a kernel, raised once per device
+template <bool NV, bool WIDE, bool INLINE>
+static cudaError_t sk_prepare(int dev) {
+  static std::atomic<bool> done[kMaxDev];
+  if (dev < kMaxDev && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(fp4_skinny_kernel<NV, WIDE, INLINE>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, sk_budget(WIDE));
+  if (e == cudaSuccess && dev < kMaxDev) done[dev].store(true, std::memory_order_relaxed);
+  return e;
+}
+
+// Shape of the launch: CL, the CTAs that share a row block.  Costs in units of a K tile (about 0.37 us), fitted to a sweep
+// of CL over 1, 8 and 16 rows and six weight sizes: each round of blocks costs a CTA its tiles, a round after the first 4
+// more and 0.08 for each row and CTA of the cluster (its reduction is not hidden), the last reduction 0.047.  A cluster
+// launch keeps an eighth of the room free: with all of it in use, a CTA of a neighbouring kernel makes one cluster wait
+// (32 clusters of 8 where 33 fit: 9.5 us, or 15.6).
+template <bool NV, bool WIDE, bool INLINE>
+static cudaError_t sk_plan(int M, int64_t N, int K, int dev, SkPlan& b, double& cost) {
+  constexpr int kSB = Fmt<NV>::kScaleBytes;
+  b = SkPlan{};
+  b.blocks = (int)((N + 127) / 128);
   b.KT = tiles_k(K);
-  b.mp = M;
   b.ncol = std::max(16, (M * kTerms + 15) / 16 * 16);
-  const int slots = (WIDE ? 1 : 2) * sms;
-  long best = -1;
+  const int xtile = b.ncol * 128 + (b.ncol > 128 ? 2 : 1) * kSB;
+  b.stage_bytes = (kTileBytes + kSB + (INLINE ? 0 : xtile) + 1023) / 1024 * 1024;
   for (int cl = 1; cl <= 8 && cl <= b.KT; ++cl) {
     const int per = (b.KT + cl - 1) / cl;
     if ((b.KT + per - 1) / per != cl) continue;       // a CTA of the cluster would have no tile
-    const int clusters = std::min(b.blocks, std::max(1, slots / cl));
-    const long steps = (long)((b.blocks + clusters - 1) / clusters) * (per + 1);
-    if (best < 0 || steps < best) {
-      best = steps;
+    if (INLINE && M * per * 16 > kEpi * 32) continue;
+    int active = 0;
+    const cudaError_t e = sk_active<WIDE>(dev, cl, &active);
+    if (e != cudaSuccess) return e;
+    if (cl > 1) active -= active / 8;
+    const int xbytes = INLINE ? (per * xtile + 1023) / 1024 * 1024 : 0;
+    const int stages = std::min(8, (sk_budget(WIDE) - 1024 - xbytes - sk_recv_bytes(cl, M)) / b.stage_bytes);
+    if (stages < 2) continue;
+    const int clusters = std::min(b.blocks, active), rounds = (b.blocks + clusters - 1) / clusters;
+    const double c = rounds * per + (rounds - 1) * (4 + 0.08 * M * cl) + 0.047 * M * cl;
+    if (b.CL == 0 || c < cost) {
+      cost = c;
       b.CL = cl;
       b.per = per;
       b.clusters = clusters;
+      b.stages = stages;
+      b.xbytes = xbytes;
     }
   }
-  constexpr int kSB = Fmt<NV>::kScaleBytes;
-  b.stage_bytes = (kTileBytes + b.ncol * 128 + kSB + (b.ncol > 128 ? 2 : 1) * kSB + 1023) / 1024 * 1024;
-  return b;
+  return b.CL ? cudaSuccess : cudaErrorInvalidConfiguration;
 }
-static int sk_recv_bytes(const SkPlan& b) { return 2 * b.CL * b.mp * 2 * ((64 + b.CL - 1) / b.CL) * 4; }
 
-template <bool NV, bool WIDE>
-static cudaError_t launch_skinny(const Fp4SkinnyArgs& p, int sms, cudaStream_t st) {
-  SkPlan pl = sk_plan<NV, WIDE>(p.mode == GEMV_SWIGLU ? (p.width + 63) / 64 * 128 : p.N, p.K, p.M, sms);
-  auto kern = fp4_skinny_kernel<NV, WIDE>;
-  const int budget = (WIDE ? 225 : 112) * 1024 - 1024 - sk_recv_bytes(pl);
-  pl.stages = std::min(8, budget / pl.stage_bytes);
-  if (pl.stages < 2) return cudaErrorInvalidConfiguration;
-  const int smem = pl.stages * pl.stage_bytes + sk_recv_bytes(pl) + 1024;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <bool NV, bool WIDE, bool INLINE>
+static cudaError_t launch_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  SkPlan b;
+  double cost;
+  if (e == cudaSuccess) e = sk_prepare<NV, WIDE, INLINE>(dev);
+  if (e == cudaSuccess) e = sk_plan<NV, WIDE, INLINE>(p.M, p.N, p.K, dev, b, cost);
   if (e != cudaSuccess) return e;
+  const int smem = b.xbytes + b.stages * b.stage_bytes + sk_recv_bytes(b.CL, p.M) + 1024;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(pl.clusters * pl.CL);
+  cfg.gridDim = dim3(b.clusters * b.CL);
   cfg.blockDim = dim3(kSkThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   int na = 0;
-  if (pl.CL > 1) {
+  if (b.CL > 1) {
     at[na].id = cudaLaunchAttributeClusterDimension;
-    at[na].val.clusterDim.x = pl.CL;
+    at[na].val.clusterDim.x = b.CL;
     at[na].val.clusterDim.y = 1;
     at[na].val.clusterDim.z = 1;
     ++na;
@@ -479,7 +645,24 @@ static cudaError_t launch_skinny(const Fp4SkinnyArgs& p, int sms, cudaStream_t s
   }
   cfg.attrs = at;
   cfg.numAttrs = na;
-  return cudaLaunchKernelEx(&cfg, kern, p, pl);
+  return cudaLaunchKernelEx(&cfg, fp4_skinny_kernel<NV, WIDE, INLINE>, p, b);
+}
+
+// a launch of fp4_expand costs about 3 tiles, so a plan with the expansion in the kernel may be that much worse
+template <bool NV>
+static bool expand_inline_t(int M, int64_t N, int K) {
+  int dev = 0;
+  SkPlan b;
+  double in = 0, sep = 0;
+  return M <= 8 && cudaGetDevice(&dev) == cudaSuccess &&
+         sk_plan<NV, false, true>(M, N, K, dev, b, in) == cudaSuccess &&
+         sk_plan<NV, false, false>(M, N, K, dev, b, sep) == cudaSuccess && in <= sep + 3;
+}
+
+template <bool NV>
+static cudaError_t skinny_t(const Fp4SkinnyArgs& p, cudaStream_t st) {
+  if (p.x) return launch_skinny<NV, false, true>(p, st);
+  return p.M <= 16 ? launch_skinny<NV, false, false>(p, st) : launch_skinny<NV, true, false>(p, st);
 }
 
 }  // namespace fp4
@@ -488,6 +671,10 @@ static cudaError_t launch_skinny(const Fp4SkinnyArgs& p, int sms, cudaStream_t s
 using namespace g53;
 
 int g53_fp4_terms() { return fp4::kTerms; }
+
+bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv) {
+  return nv ? fp4::expand_inline_t<true>(M, N, K) : fp4::expand_inline_t<false>(M, N, K);
+}
 
 cudaError_t g53_fp4_expand(const Fp4ExpandArgs& p, cudaStream_t st) {
   if (p.M < 1 || p.M > 32 || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
@@ -498,12 +685,7 @@ cudaError_t g53_fp4_expand(const Fp4ExpandArgs& p, cudaStream_t st) {
 
 cudaError_t g53_fp4_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
   if (p.M < 1 || p.M > 32 || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
-  int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return e;
-  if (p.nv) return p.M <= 16 ? fp4::launch_skinny<true, false>(p, sms, st) : fp4::launch_skinny<true, true>(p, sms, st);
-  return p.M <= 16 ? fp4::launch_skinny<false, false>(p, sms, st) : fp4::launch_skinny<false, true>(p, sms, st);
+  return p.nv ? fp4::skinny_t<true>(p, st) : fp4::skinny_t<false>(p, st);
 }
 
 cudaError_t g53_fp4_skinny_error(int* code) {

@@ -415,6 +415,8 @@ cudaError_t g53_fp4_dequant(const Fp4DequantArgs& p, cudaStream_t st);
 
 // Expansion of M <= 32 bf16 rows into g53_fp4_terms() 4-bit rows each (fp4_skinny.cu): image rows terms * m + t
 int g53_fp4_terms();
+// whether the product expands these rows itself, without a launch of g53_fp4_expand
+bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv);
 struct Fp4ExpandArgs {
   const __nv_bfloat16* x; int64_t ldx;
   int M, K, nv;
@@ -424,14 +426,15 @@ struct Fp4ExpandArgs {
 };
 cudaError_t g53_fp4_expand(const Fp4ExpandArgs& p, cudaStream_t st);
 
-// y[M, N] (mode) = x[M, K] @ W4[N, K]^T for expanded rows, M <= 32 (fp4_skinny.cu).  GEMV_SWIGLU: W4 is a gate/up image
+// y[M, N] (mode) = x[M, K] @ W4[N, K]^T for M <= 32 (fp4_skinny.cu), x as rows or expanded.  GEMV_SWIGLU: W4 is a gate/up image
 // (64 gate rows, then their 64 up rows, per 128-row block), y [M, width] bf16
 struct Fp4SkinnyArgs {
+  const __nv_bfloat16* x; int64_t ldx; int xvec;   // the rows themselves (expanded by the kernel), or null:
   const uint8_t* x_codes; const uint8_t* x_scales; const float* x_factor;
   const uint8_t* codes; const uint8_t* scales; const float* row_scale;
   int nv;
   void* y; int64_t ldy;
-  int M, N, K;
+  int M, N, K;                         // N: rows of W4 (of the gate/up image, whole blocks)
   int width;                           // GEMV_SWIGLU: columns of y
   int mode;
   float limit;

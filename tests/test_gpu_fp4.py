@@ -70,17 +70,15 @@ def sums_tol(a, w):
 
 
 def act_tol(x, w, fmt):
-    """Bound of what the 8-term expansion of 16-bit activations leaves out (x, w in 64 bits).  nvfp4: the block scale is
-    within 1/16 of a sixth of the maximum, and rounding leaves at most one scale: (17/96)^8 < 2^-19 of the block's
-    maximum; a block whose scale underflows e4m3 waits for a later term, whose row factor is smaller: 2^-31 of the row's
-    maximum.  mxfp4: the first scale is under a third of the maximum, each next one a quarter of the last: 4^-7 / 3 <
-    2^-15."""
+    """Bound of what the expansion of 16-bit activations leaves out (x, w in 64 bits): a block's elements are rounded to
+    multiples of 2^(e-21), 2^e the binade of its largest, so by at most 2^-22 of that; in nvfp4 a block more than 2^17
+    below the row's largest is rounded as one at 2^-17 (2^-39 of the row's largest)."""
     blk = 16 if fmt == "nvfp4" else 32
     amax = x.abs().view(x.shape[0], -1, blk).amax(-1)
     wsum = w.abs().view(w.shape[0], -1, blk).sum(-1)
-    if fmt == "mxfp4":
-        return 2.0 ** -15 * amax @ wsum.t()
-    return (2.0 ** -19 * amax + 2.0 ** -31 * amax.amax(1, keepdim=True)) @ wsum.t()
+    if fmt == "nvfp4":
+        amax = torch.maximum(amax, 2.0 ** -17 * amax.amax(1, keepdim=True))
+    return 2.0 ** -22 * amax @ wsum.t()
 
 
 def half(dtype):
