@@ -83,11 +83,10 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t amax_bits) {
 }
 
 // nvfp4 row scale 2^k from the bits of the row's largest magnitude: the smallest with amax <= 448 * 6 * 2^k =
-// 1.3125 * 2^(k+11), within the normal range.  The block scale then uses e4m3's full range and the row scale costs no
-// rounding.
+// 1.3125 * 2^(k+11), and not below 2^-100.  The block scale then uses e4m3's full range and the row scale costs no rounding.
 __host__ __device__ __forceinline__ int nv_row_exp(uint32_t amax_bits) {
   const int k = (int)(amax_bits >> 23) - 127 - 11 + ((amax_bits & 0x7fffffu) > 0x280000u ? 1 : 0);
-  return k < -126 ? -126 : k;
+  return k < -100 ? -100 : k;
 }
 // e4m3 block scale: amax * 2^-k / 6, rounded to nearest even.  An IEEE division: amax * 2^-k = 6 * (a tie between two
 // e4m3 values) happens with 16-bit inputs, and the quotient is then exact.
@@ -96,13 +95,19 @@ __device__ __forceinline__ uint32_t nv_scale(float amax_scaled) {
   return (uint32_t)v.__x;
 }
 
-// x * inv rounded to 16 significant bits (Veltkamp's split), inv the rounded reciprocal of the block scale s.  For x of
-// at most 11 significant bits (bf16, f16) and s of at most 4, x / s either equals a border between two codes or is at
-// least 2^-11 of it away, so the error of 2^-23 that the reciprocal adds is removed and ties fall as they would with
-// the exact quotient.
-__device__ __forceinline__ float snap16(float q) {
-  const float c = __fmul_rn(q, 257.f);               // no contraction into an fma, which would keep every bit
-  return __fsub_rn(c, __fsub_rn(c, q));
+// x * inv on the grid of 2^-15, for |x * inv| < 8 and inv the rounded reciprocal of a block scale s (times a power of
+// two).  For x of at most 11 significant bits (bf16, f16) and s of at most 4, x / s either equals a border between two
+// codes (a multiple of 1/4) or is at least 2^-11 of it, so 2^-13, away: the error that the reciprocal adds (below 2^-20) is
+// removed, nothing crosses a border, and ties fall as they would with the exact quotient.  Two instructions.
+__device__ __forceinline__ float scaled_on_grid(float x, float inv) {
+  return __fsub_rn(__fmaf_rn(x, inv, 384.f), 384.f);
+}
+
+// largest of the magnitudes of 16-bit floats, in pairs
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 }  // namespace fp4

@@ -31,47 +31,70 @@ cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 std::string num(int64_t v) { return std::to_string(v); }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// a 4-bit matrix: its arrays and shape, checked once when it is made
-struct Matrix4 {
-  Tensor codes, scales;
-  OptT row_scale;
-  int64_t rows, k;
-  bool nv;
+int64_t n_tiles(int64_t rows, int64_t k) { return ((rows + kTileRows - 1) / kTileRows) * ((k + kTileK - 1) / kTileK); }
+int64_t scale_bytes(bool nv) { return kTileRows * (kTileK / (nv ? 16 : 32)); }
 
-  Matrix4(Tensor c, Tensor s, OptT r, int64_t rows_, int64_t k_, bool nv_)
-      : codes(std::move(c)), scales(std::move(s)), row_scale(std::move(r)), rows(rows_), k(k_), nv(nv_) {
+// a 4-bit matrix: its arrays and shape, checked once when it is made.  Matrices made here keep their three arrays in one
+// buffer; the views that Python sees are made when asked for
+struct Matrix4 {
+  Tensor parts[3];                     // codes, scales, row scale; or the one buffer in parts[0]
+  bool whole = false;
+  int64_t rows = 0, k = 0;
+  bool nv = false;
+  uint8_t* codes = nullptr;
+  uint8_t* scales = nullptr;
+  float* row_scale = nullptr;
+
+  static void check_shape(int64_t rows, int64_t k, bool nv) {
     const int64_t block = nv ? 16 : 32;
     TORCH_CHECK(rows >= 1 && k >= block && k % block == 0, "Matrix4: rows >= 1 and K a multiple of ", num(block), ", got [",
                 num(rows), ", ", num(k), "]");
     TORCH_CHECK(rows < (int64_t)1 << 31 && k < (int64_t)1 << 31, "Matrix4: at most 2^31 - 1 rows and columns");
-    const int64_t tiles = ((rows + kTileRows - 1) / kTileRows) * ((k + kTileK - 1) / kTileK);
-    TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kByte && codes.is_contiguous() &&
-                    codes.numel() == tiles * kTileBytes && aligned16(codes.data_ptr()),
-                "Matrix4: codes must be ", num(tiles * kTileBytes), " contiguous, 16-byte aligned uint8 on a CUDA device");
-    TORCH_CHECK(scales.device() == codes.device() && scales.scalar_type() == at::kByte && scales.is_contiguous() &&
-                    scales.numel() == tiles * kTileRows * (kTileK / block) && aligned16(scales.data_ptr()),
-                "Matrix4: scales must be ", num(tiles * kTileRows * (kTileK / block)),
-                " contiguous, 16-byte aligned uint8 on the codes' device");
-    TORCH_CHECK(nv == row_scale.has_value(), "Matrix4: nvfp4 has a row scale, mxfp4 none");
-    if (nv)
-      TORCH_CHECK(row_scale->device() == codes.device() && row_scale->scalar_type() == at::kFloat &&
-                      row_scale->is_contiguous() && row_scale->numel() >= rows && aligned16(row_scale->data_ptr()),
-                  "Matrix4: row_scale must be fp32 [rows], contiguous, 16-byte aligned, on the codes' device");
   }
-  const uint8_t* c() const { return codes.data_ptr<uint8_t>(); }
-  const uint8_t* s() const { return scales.data_ptr<uint8_t>(); }
-  const float* r() const { return nv ? row_scale->data_ptr<float>() : nullptr; }
+  Matrix4(int64_t rows_, int64_t k_, bool nv_, const Tensor& like) : whole(true), rows(rows_), k(k_), nv(nv_) {
+    check_shape(rows, k, nv);
+    const int64_t c = n_tiles(rows, k) * kTileBytes, s = n_tiles(rows, k) * scale_bytes(nv);
+    parts[0] = at::empty({c + s + (nv ? 4 * rows : 0)}, like.options().dtype(at::kByte));
+    codes = parts[0].data_ptr<uint8_t>();
+    scales = codes + c;
+    if (nv) row_scale = reinterpret_cast<float*>(scales + s);
+  }
+  Matrix4(const Tensor& c, const Tensor& s, const OptT& r, int64_t rows_, int64_t k_, bool nv_)
+      : rows(rows_), k(k_), nv(nv_) {
+    check_shape(rows, k, nv);
+    const int64_t t = n_tiles(rows, k);
+    TORCH_CHECK(c.is_cuda() && c.scalar_type() == at::kByte && c.is_contiguous() && c.numel() == t * kTileBytes &&
+                    aligned16(c.data_ptr()),
+                "Matrix4: codes must be ", num(t * kTileBytes), " contiguous, 16-byte aligned uint8 on a CUDA device");
+    TORCH_CHECK(s.device() == c.device() && s.scalar_type() == at::kByte && s.is_contiguous() &&
+                    s.numel() == t * scale_bytes(nv) && aligned16(s.data_ptr()),
+                "Matrix4: scales must be ", num(t * scale_bytes(nv)),
+                " contiguous, 16-byte aligned uint8 on the codes' device");
+    TORCH_CHECK(nv == r.has_value(), "Matrix4: nvfp4 has a row scale, mxfp4 none");
+    if (nv) {
+      TORCH_CHECK(r->device() == c.device() && r->scalar_type() == at::kFloat && r->is_contiguous() &&
+                      r->numel() == rows && aligned16(r->data_ptr()),
+                  "Matrix4: row_scale must be fp32 [rows], contiguous, 16-byte aligned, on the codes' device");
+      parts[2] = *r;
+      row_scale = r->data_ptr<float>();
+    }
+    parts[0] = c;
+    parts[1] = s;
+    codes = c.data_ptr<uint8_t>();
+    scales = s.data_ptr<uint8_t>();
+  }
+  at::Device device() const { return parts[0].device(); }
+  Tensor codes_view() const { return whole ? parts[0].narrow(0, 0, n_tiles(rows, k) * kTileBytes) : parts[0]; }
+  Tensor scales_view() const {
+    const int64_t t = n_tiles(rows, k);
+    return whole ? parts[0].narrow(0, t * kTileBytes, t * scale_bytes(nv)) : parts[1];
+  }
+  OptT row_scale_view() const {
+    if (!nv) return c10::nullopt;
+    const int64_t t = n_tiles(rows, k);
+    return whole ? parts[0].narrow(0, t * (kTileBytes + scale_bytes(nv)), 4 * rows).view(at::kFloat) : parts[2];
+  }
 };
-
-Matrix4 empty4(int64_t rows, int64_t k, bool nv, const Tensor& like) {
-  const int64_t block = nv ? 16 : 32;
-  const int64_t tiles = ((rows + kTileRows - 1) / kTileRows) * ((k + kTileK - 1) / kTileK);
-  const auto u8 = like.options().dtype(at::kByte);
-  Tensor c = torch::empty({tiles * kTileBytes}, u8), s = torch::empty({tiles * kTileRows * (kTileK / block)}, u8);
-  OptT r;
-  if (nv) r = torch::empty({rows}, like.options().dtype(at::kFloat));
-  return Matrix4(std::move(c), std::move(s), std::move(r), rows, k, nv);
-}
 
 void check_x(const Tensor& x, const char* op) {
   TORCH_CHECK(x.is_cuda(), op, ": x must be a CUDA tensor");
@@ -83,7 +106,7 @@ Matrix4 quantize(const Tensor& x, bool nv) {
   check_x(x, "quantize4");
   TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "quantize4: x must be bf16 or f16");
   const c10::cuda::CUDAGuard guard(x.device());
-  Matrix4 m = empty4(x.size(0), x.size(1), nv, x);
+  Matrix4 m(x.size(0), x.size(1), nv, x);
   Fp4QuantArgs a{};
   a.x = x.data_ptr();
   a.ldx = x.stride(0);
@@ -92,18 +115,18 @@ Matrix4 quantize(const Tensor& x, bool nv) {
   a.nv = nv;
   a.f16 = x.scalar_type() == at::kHalf;
   a.vec = aligned16(a.x) && a.ldx % 8 == 0;
-  a.codes = m.codes.data_ptr<uint8_t>();
-  a.scales = m.scales.data_ptr<uint8_t>();
-  a.row_scale = nv ? m.row_scale->data_ptr<float>() : nullptr;
+  a.codes = m.codes;
+  a.scales = m.scales;
+  a.row_scale = m.row_scale;
   ok(g53_fp4_quantize(a, stream()), "fp4_quantize");
   return m;
 }
 
 void dequant(const Matrix4& m, const Tensor& y, int64_t il) {
   Fp4DequantArgs a{};
-  a.codes = m.c();
-  a.scales = m.s();
-  a.row_scale = m.r();
+  a.codes = m.codes;
+  a.scales = m.scales;
+  a.row_scale = m.row_scale;
   a.R = m.rows;
   a.K = m.k;
   a.nv = m.nv;
@@ -115,21 +138,25 @@ void dequant(const Matrix4& m, const Tensor& y, int64_t il) {
   ok(g53_fp4_dequant(a, stream()), "fp4_dequant");
 }
 
-void dequantize(const Matrix4& m, const Tensor& y) {
-  TORCH_CHECK(y.device() == m.codes.device(), "dequantize4: the output must be on the matrix's device");
+Tensor dequantize(const Matrix4& m, const OptT& out, at::ScalarType dtype) {
+  const c10::cuda::CUDAGuard guard(m.device());
+  TORCH_CHECK(out.has_value() || dtype == at::kBFloat16 || dtype == at::kHalf || dtype == at::kFloat,
+              "dequantize4: the output must be bf16, f16 or fp32");
+  const Tensor y = out.has_value() ? *out : at::empty({m.rows, m.k}, m.parts[0].options().dtype(dtype));
+  TORCH_CHECK(y.device() == m.device(), "dequantize4: the output must be on the matrix's device");
   TORCH_CHECK(y.scalar_type() == at::kBFloat16 || y.scalar_type() == at::kHalf || y.scalar_type() == at::kFloat,
               "dequantize4: the output must be bf16, f16 or fp32");
   TORCH_CHECK(y.dim() == 2 && y.size(0) == m.rows && y.size(1) == m.k && y.stride(1) == 1 &&
                   (m.rows == 1 || y.stride(0) >= m.k),
               "dequantize4: the output must be [", num(m.rows), ", ", num(m.k), "], rows contiguous and apart");
-  const c10::cuda::CUDAGuard guard(y.device());
   dequant(m, y, 0);
+  return y;
 }
 
 void check_xy(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t mode, const char* op) {
   check_x(x, op);
   TORCH_CHECK(x.scalar_type() == at::kBFloat16, op, ": x must be bf16");
-  TORCH_CHECK(x.device() == w.codes.device() && y.device() == x.device(), op, ": x, y and the weights must be on one device");
+  TORCH_CHECK(x.device() == w.device() && y.device() == x.device(), op, ": x, y and the weights must be on one device");
   TORCH_CHECK(x.size(1) == w.k, op, ": K mismatch: x ", num(x.size(1)), ", weights ", num(w.k));
   TORCH_CHECK(mode == GEMV_BF16 || mode == GEMV_F32 || mode == GEMV_F32_ACC, op, ": mode must be GEMV_BF16, GEMV_F32 or "
               "GEMV_F32_ACC");
@@ -142,7 +169,7 @@ void check_xy(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int
 
 // all rows of x through the small-M kernel, kSkinnyRows at a time
 void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t width, int64_t mode, double limit) {
-  const int64_t K = w.k, sb = kTileRows * (kTileK / (w.nv ? 16 : 32));
+  const int64_t K = w.k, sb = scale_bytes(w.nv);
   for (int64_t m0 = 0; m0 < x.size(0); m0 += kSkinnyRows) {
     const int64_t m = std::min(kSkinnyRows, x.size(0) - m0);
     const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()) + m0 * x.stride(0);
@@ -154,8 +181,8 @@ void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64
       a.ldx = x.stride(0);
       a.xvec = vec;
     } else {
-      const int64_t tiles = (m * g53_fp4_terms() + kTileRows - 1) / kTileRows * ((K + kTileK - 1) / kTileK);
-      buf = torch::empty({tiles * (kTileBytes + sb) + m * 4}, x.options().dtype(at::kByte));
+      const int64_t tiles = n_tiles(m * g53_fp4_terms(), K);
+      buf = at::empty({tiles * (kTileBytes + sb) + m * 4}, x.options().dtype(at::kByte));
       uint8_t* b = buf.data_ptr<uint8_t>();
       Fp4ExpandArgs e{};
       e.x = rows;
@@ -169,9 +196,9 @@ void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64
       a.x_factor = e.factor = reinterpret_cast<float*>(b + tiles * (kTileBytes + sb));
       ok(g53_fp4_expand(e, stream()), "fp4_expand");
     }
-    a.codes = w.c();
-    a.scales = w.s();
-    a.row_scale = w.r();
+    a.codes = w.codes;
+    a.scales = w.scales;
+    a.row_scale = w.row_scale;
     a.nv = w.nv;
     a.y = reinterpret_cast<uint8_t*>(y.data_ptr()) + m0 * y.stride(0) * y.element_size();
     a.ldy = y.stride(0);
@@ -189,7 +216,7 @@ void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64
 // the bf16 tcgen05 GEMM
 void gemm_exact(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t il, int64_t mode, double limit) {
   Tensor xx = aligned16(x.data_ptr()) && x.stride(0) % 8 == 0 ? x : x.contiguous().clone();
-  Tensor wb = torch::empty({n, w.k}, x.options());
+  const Tensor wb = at::empty({n, w.k}, x.options());
   dequant(w, wb, il);
   GemmArgs p{};
   p.a = xx.data_ptr();
@@ -209,13 +236,13 @@ void gemm_exact(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, i
 
 Fp4GemmArgs gemm_args(const Matrix4& a, const Matrix4& w, int64_t mode) {
   Fp4GemmArgs p{};
-  p.a_codes = a.c();
-  p.a_scales = a.s();
-  p.a_row = a.r();
+  p.a_codes = a.codes;
+  p.a_scales = a.scales;
+  p.a_row = a.row_scale;
   p.a_const = 1.f;
-  p.b_codes = w.c();
-  p.b_scales = w.s();
-  p.b_row = w.r();
+  p.b_codes = w.codes;
+  p.b_scales = w.scales;
+  p.b_row = w.row_scale;
   p.nv = w.nv;
   p.M = (int)a.rows;
   p.N = (int)w.rows;
@@ -247,12 +274,12 @@ int row_exp(float bound) {
   uint32_t b;
   std::memcpy(&b, &bound, 4);
   const int k = (int)(b >> 23) - 127 - 11 + ((b & 0x7fffffu) > 0x280000u ? 1 : 0);
-  return std::max(k, -126);
+  return std::max(k, -100);
 }
 
 void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& y, double limit, int64_t mode, bool act4) {
   const int64_t W = down.k;
-  TORCH_CHECK(gu.nv == down.nv && gu.codes.device() == down.codes.device(), "mlp4: both matrices in one format, on one device");
+  TORCH_CHECK(gu.nv == down.nv && gu.device() == down.device(), "mlp4: both matrices in one format, on one device");
   TORCH_CHECK(W % 32 == 0 && gu.rows == (W + 63) / 64 * 128, "mlp4: the gate/up image must have ", num((W + 63) / 64 * 128),
               " rows for a width of ", num(W), " (a multiple of 32)");
   check_xy(x, gu, y, down.rows, mode, "mlp4");
@@ -266,12 +293,12 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
   const c10::cuda::CUDAGuard guard(x.device());
   if (four) {
     const Matrix4 a = quantize(x, gu.nv);
-    Matrix4 h = empty4(M, W, gu.nv, x);
+    const Matrix4 h(M, W, gu.nv, x);
     Fp4GemmArgs p = gemm_args(a, gu, GEMV_SWIGLU);
     p.limit = (float)limit;
     p.width = (int)W;
-    p.out_codes = h.codes.data_ptr<uint8_t>();
-    p.out_scales = h.scales.data_ptr<uint8_t>();
+    p.out_codes = h.codes;
+    p.out_scales = h.scales;
     p.h_exp = gu.nv ? row_exp(l2) : 0;
     ok(g53_fp4_gemm(p, stream()), "fp4_gemm");
     Fp4GemmArgs d = gemm_args(h, down, mode);
@@ -282,7 +309,7 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
     ok(g53_fp4_gemm(d, stream()), "fp4_gemm");
     return;
   }
-  const Tensor h = torch::empty({M, W}, x.options());
+  const Tensor h = at::empty({M, W}, x.options());
   if (M >= kGemmRows) {
     gemm_exact(x, gu, h, 2 * W, W, GEMV_SWIGLU_F32, limit);
     gemm_exact(h, down, y, down.rows, 0, mode, 0.0);
@@ -305,10 +332,10 @@ int64_t error(int64_t device) {
 void register_fp4(pybind11::module& m) {
   namespace py = pybind11;
   py::class_<Matrix4>(m, "Matrix4")
-      .def(py::init<Tensor, Tensor, OptT, int64_t, int64_t, bool>())
-      .def_readonly("codes", &Matrix4::codes)
-      .def_readonly("scales", &Matrix4::scales)
-      .def_readonly("row_scale", &Matrix4::row_scale)
+      .def(py::init<const Tensor&, const Tensor&, const OptT&, int64_t, int64_t, bool>())
+      .def_property_readonly("codes", &Matrix4::codes_view)
+      .def_property_readonly("scales", &Matrix4::scales_view)
+      .def_property_readonly("row_scale", &Matrix4::row_scale_view)
       .def_readonly("rows", &Matrix4::rows)
       .def_readonly("k", &Matrix4::k)
       .def_readonly("nv", &Matrix4::nv);

@@ -9,10 +9,11 @@
 //   warp 0    producer: fills a 4-stage (BN 256) ring, continuously across tiles
 //   warp 1    allocates TMEM; one thread copies the block scales of the stage to TMEM (tcgen05.cp, executed in order with
 //             the mma of the same thread) and issues the four K = 64 mma of the stage
-//   warps 2-5 epilogue: tcgen05.ld, row scales, output
+//   warps 2-9 epilogue: tcgen05.ld, row scales, output (four warps, one per scheduler, take longer over the SwiGLU epilogue
+//             than the main loop: 700 us instead of 340 for 8192 x 24576 x 4096)
 // TMEM (512 columns): scales at 448..495; with BN = 256 the two accumulators are columns 0..255 and 192..447.  They share
-// 64 columns, which the epilogue of a tile reads first and then hands back, so the main loop of the next tile waits
-// for a quarter of the epilogue's loads only.
+// 64 columns, which the epilogue of a tile reads first and then hands back, so the main loop of the next tile waits for
+// a quarter of the epilogue's loads only.
 //
 // GEMV_SWIGLU: W4 is a gate/up image (per 128-row block 64 gate rows, then their 64 up rows); the epilogue forms
 // silu(min(g, L)) * clip(u, -L, L) in fp32 and quantises it in place: a thread holds 32 consecutive activations of one row,
@@ -23,6 +24,7 @@
 // Waits are bounded; a timeout sets the error word, the roles stop issuing, wait for what they have in flight, and the
 // TMEM is freed.
 #include <algorithm>
+#include <atomic>
 #include "fp4.cuh"
 #include "fp4_tc.cuh"
 #include "launchers.h"
@@ -32,7 +34,8 @@ namespace fp4 {
 
 __device__ int g_gemm_err = 0;
 
-constexpr int kGemmThreads = 192;
+constexpr int kEpiWarps = 8;
+constexpr int kGemmThreads = 64 + kEpiWarps * 32;
 constexpr int kBandM = 8;
 constexpr uint32_t kSfA = 448, kSfB = 464;            // TMEM columns of the scales
 
@@ -117,15 +120,25 @@ __device__ __forceinline__ void swiglu32(const Fp4GemmArgs& p, int row, int j0, 
                                          float (&u)[32]) {
   const float L = p.limit;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    float g = v[i], w = u[i];
+  for (int i = 0; i < 32; i += 4) {
+    float4 sg = make_float4(1.f, 1.f, 1.f, 1.f), su = sg;
     if constexpr (NV) {
-      g *= rs * p.b_row[r0 + i];
-      w *= rs * p.b_row[r0 + 64 + i];
+      sg = __ldg(reinterpret_cast<const float4*>(p.b_row + r0 + i));
+      su = __ldg(reinterpret_cast<const float4*>(p.b_row + r0 + 64 + i));
     }
-    g = g > L ? L : g;                                // written so that a NaN stays one
-    w = w > L ? L : w < -L ? -L : w;
-    v[i] = siluf_(g) * w;
+    const float gs[4] = {sg.x, sg.y, sg.z, sg.w}, us[4] = {su.x, su.y, su.z, su.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float g = v[i + k], w = u[i + k];
+      if constexpr (NV) {
+        g *= rs * gs[k];
+        w *= rs * us[k];
+      }
+      g = g > L ? L : g;                              // written so that a NaN stays one
+      w = w > L ? L : w < -L ? -L : w;
+      // g <= L; exp(-g) that overflows leaves g / inf = -0, and __fdividef is 0 there too
+      v[i + k] = __fdividef(g, 1.f + __expf(-g)) * w;
+    }
   }
   const int rr = row % kTileRows, kt = j0 / kTileK, c = (j0 % kTileK) / 32;
   const int64_t tile = (int64_t)(row / kTileRows) * tiles_k(p.width) + kt;
@@ -194,7 +207,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
     }
     for (int b = 0; b < 2; ++b) {
       tc::bar_init(&tfull[b], 1);
-      tc::bar_init(&tempty[b], 4);
+      tc::bar_init(&tempty[b], kEpiWarps);
     }
     tc::bar_init(&drain, 1);
     fail_s = 0;
@@ -289,7 +302,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
     }
     __syncwarp();
   } else {
-    const int quad = warp & 3;
+    // two warps per TMEM lane quadrant; `part` 0 takes the half of the tile with the shared columns.  Its arrival on
+    // tempty says that those are read; that of part 1, that it is done with the tile before
+    const int quad = warp & 3, part = (warp - 2) >> 2;
     uint32_t tl = 0;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++tl) {
       const uint32_t buf = tl & 1;
@@ -306,39 +321,48 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
         __syncwarp();
         if (lane == 0) tc::bar_arrive(&tempty[buf]);
       };
-      // units of 64 columns; the one in the shared columns first
+      if (BN == 256 && part == 1) release();
       if constexpr (SWI) {
-#pragma unroll 1
-        for (int i = 0; i < C::kNB; ++i) {
-          const int blk = C::kNB == 2 ? (buf == 0 ? 1 - i : i) : 0;
-          const int nblk = nt * C::kNB + blk;
-          // the half of the pair that lies in the shared columns: up (buffer 0, block 1) or gate (buffer 1, block 0)
+        const int wide = ((p.width + 63) / 64) * 64;
+        if constexpr (BN == 256) {
+          // a block (64 gate, 64 up columns) per part.  The shared columns are the up half of block 1 (buffer 0) or the gate
+          // half of block 0 (buffer 1)
+          const int blk = buf == 0 ? 1 - part : part;
+          const int nblk = nt * 2 + blk;
           const uint32_t first = buf == 0 ? 64u : 0u;
           float x0[32], x1[32], w[32];
           tc::tmem_ld32(base + blk * 128 + first, x0);
           tc::tmem_ld32(base + blk * 128 + first + 32, x1);
-          if (C::kNB == 2 && i == 0) release();
+          if (part == 0) release();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             tc::tmem_ld32(base + blk * 128 + (64u - first) + h * 32, w);
             const int j0 = nblk * 64 + h * 32;
-            if (live && j0 < ((p.width + 63) / 64) * 64) {
+            if (live && j0 < wide) {
               const int r0 = nblk * 128 + h * 32;
               if (buf == 0) swiglu32<NV>(p, row, j0, r0, rs, w, h == 0 ? x0 : x1);
               else swiglu32<NV>(p, row, j0, r0, rs, h == 0 ? x0 : x1, w);
             }
           }
-          if (C::kNB == 1) release();
+        } else {
+          float g[32], u[32];
+          tc::tmem_ld32(base + part * 32, g);
+          tc::tmem_ld32(base + 64 + part * 32, u);
+          release();
+          const int j0 = nt * 64 + part * 32;
+          if (live && j0 < wide) swiglu32<NV>(p, row, j0, nt * 128 + part * 32, rs, g, u);
         }
       } else {
         const int n0 = nt * BN;
+        constexpr int kUnits = BN / 128;              // units of 64 columns per part
 #pragma unroll 1
-        for (int i = 0; i < BN / 64; ++i) {
-          const int u = BN == 256 && buf == 0 ? (i + 3) & 3 : i;
+        for (int i = 0; i < kUnits; ++i) {
+          // buffer 0 of BN 256: units 3, 2 and 0, 1
+          const int u = BN == 256 && buf == 0 ? (part == 0 ? 3 - i : i) : part * kUnits + i;
           float x0[32], x1[32];
           tc::tmem_ld32(base + u * 64, x0);
           tc::tmem_ld32(base + u * 64 + 32, x1);
-          if (BN == 256 ? i == 0 : i == BN / 64 - 1) release();
+          if (BN == 256 ? part == 0 && i == 0 : true) release();
           if (live && n0 + u * 64 < p.N) store32(p, row, n0 + u * 64, rs, x0);
           if (live && n0 + u * 64 + 32 < p.N) store32(p, row, n0 + u * 64 + 32, rs, x1);
         }
@@ -353,23 +377,38 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
   }
 }
 
+constexpr int kMaxDev = 64;
+
+// SMs of the current device
+static cudaError_t sm_count(int dev, int* out) {
+  static std::atomic<int> known[kMaxDev];
+  if (dev < kMaxDev && (*out = known[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  const cudaError_t e = cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess && dev < kMaxDev) known[dev].store(*out, std::memory_order_relaxed);
+  return e;
+}
+
 template <bool NV, int BN, bool SWI>
-static cudaError_t launch_gemm(const Fp4GemmArgs& p, int sms, cudaStream_t st) {
+static cudaError_t launch_gemm(const Fp4GemmArgs& p, int dev, int sms, cudaStream_t st) {
   using C = GemmCfg<NV, BN>;
   auto kern = fp4_gemm_kernel<NV, BN, SWI>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-  if (e != cudaSuccess) return e;
+  static std::atomic<bool> ready[kMaxDev];            // the shared memory limit, raised once per device
+  if (dev >= kMaxDev || !ready[dev].load(std::memory_order_relaxed)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDev) ready[dev].store(true, std::memory_order_relaxed);
+  }
   const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + BN - 1) / BN);
   kern<<<(unsigned)std::min<int64_t>(tiles, sms), kGemmThreads, C::kSmem, st>>>(p);
   return cudaGetLastError();
 }
 
 template <bool NV>
-static cudaError_t gemm_t(const Fp4GemmArgs& p, int sms, cudaStream_t st) {
+static cudaError_t gemm_t(const Fp4GemmArgs& p, int dev, int sms, cudaStream_t st) {
   const bool wide = (int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256) >= sms;
   if (p.mode == GEMV_SWIGLU)
-    return wide ? launch_gemm<NV, 256, true>(p, sms, st) : launch_gemm<NV, 128, true>(p, sms, st);
-  return wide ? launch_gemm<NV, 256, false>(p, sms, st) : launch_gemm<NV, 128, false>(p, sms, st);
+    return wide ? launch_gemm<NV, 256, true>(p, dev, sms, st) : launch_gemm<NV, 128, true>(p, dev, sms, st);
+  return wide ? launch_gemm<NV, 256, false>(p, dev, sms, st) : launch_gemm<NV, 128, false>(p, dev, sms, st);
 }
 
 }  // namespace fp4
@@ -381,12 +420,12 @@ cudaError_t g53_fp4_gemm(const Fp4GemmArgs& p, cudaStream_t st) {
   if (p.M < 1 || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = fp4::sm_count(dev, &sms);
   if (e != cudaSuccess) return e;
   Fp4GemmArgs q = p;
   const int esz = p.mode == GEMV_BF16 ? 2 : 4;
   q.vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && ((p.ldy * esz) & 15) == 0 ? 1 : 0;
-  return p.nv ? fp4::gemm_t<true>(q, sms, st) : fp4::gemm_t<false>(q, sms, st);
+  return p.nv ? fp4::gemm_t<true>(q, dev, sms, st) : fp4::gemm_t<false>(q, dev, sms, st);
 }
 
 cudaError_t g53_fp4_gemm_error_word(int** word) {

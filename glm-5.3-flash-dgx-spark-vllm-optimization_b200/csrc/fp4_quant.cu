@@ -58,13 +58,10 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(Fp4QuantArgs p) {
   };
   // bits (fp32) of the block's largest magnitude
   auto amax16 = [&](const uint32_t (&w)[8]) {
-    uint32_t lo = 0u, hi = 0u;
+    uint32_t a = w[0] & 0x7fff7fffu;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo = max(lo, w[i] & 0x7fffu);
-      hi = max(hi, w[i] & 0x7fff0000u);
-    }
-    const uint32_t m = max(lo, hi >> 16);
+    for (int i = 1; i < 8; ++i) a = max_u16x2(a, w[i] & 0x7fff7fffu);
+    const uint32_t m = max(a & 0xffffu, a >> 16);
     if constexpr (F16) {
       if (m >= 0x7c00u) return kInfBits;
       return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
@@ -113,7 +110,7 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(Fp4QuantArgs p) {
       const float a = __uint_as_float(amax) * down;
       sc = amax >= kInfBits ? 0x7fu : nv_scale(a);
       const float s = e4m3_to_f32(sc);
-      inv = s > 0.f ? __frcp_rn(s) : 0.f;
+      inv = s > 0.f ? __frcp_rn(s) * down : 0.f;      // down >= 2^-117: no underflow of note
     } else {
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));     // the other half of the 32-block
       sc = mx_scale(amax);
@@ -128,8 +125,8 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(Fp4QuantArgs p) {
         float lo, hi;
         unpack2<F16>(v[4 * h + i], lo, hi);
         if constexpr (NV) {
-          f[2 * i] = snap16(lo * down * inv);
-          f[2 * i + 1] = snap16(hi * down * inv);
+          f[2 * i] = scaled_on_grid(lo, inv);
+          f[2 * i + 1] = scaled_on_grid(hi, inv);
         } else {                                       // exact: the scale is a power of two
           f[2 * i] = lo * inv;
           f[2 * i + 1] = hi * inv;
@@ -173,29 +170,32 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(Fp4QuantArgs p) {
 // il (gate/up images, fp4 row order of pack): row 128 b + j (j < 64) is gate row 64 b + j, row 128 b + 64 + j up row
 // 64 b + j; the output rows are the (8 gate, 8 up) interleave of the 16-bit GEMM's SwiGLU epilogue, rows of gate index
 // >= il skipped.
+// CTA: 8 rows (a warp each) x 8 tiles.
+constexpr int kDqTiles = 8;
 template <bool NV, int OUT>                           // OUT 0 bf16, 1 f16, 2 fp32
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(Fp4DequantArgs p) {
   const int KT = tiles_k(p.K);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t units = (int64_t)p.R * KT;            // one unit: one row of one tile
-  const int64_t step = (int64_t)gridDim.x * 8;
-  for (int64_t u = (int64_t)blockIdx.x * 8 + warp; u < units; u += step) {
-    const int64_t row = u / KT;
-    const int kt = (int)(u - row * KT);
-    const int rr = (int)(row % kTileRows);
+  const int64_t row = (int64_t)blockIdx.x * 8 + warp;
+  if (row >= p.R) return;
+  const int rr = (int)(row % kTileRows);
+  int64_t orow = row;
+  if (p.il > 0) {
+    const int64_t j = (row / 128) * 64 + (row % 64);
+    if (j >= p.il) return;
+    orow = (j / 8) * 16 + (j % 8) + ((row % 128) >= 64 ? 8 : 0);
+  }
+  const float rs = NV ? __ldg(p.row_scale + row) : 1.f;
+  const int kt1 = min(KT, ((int)blockIdx.y + 1) * kDqTiles);
+#pragma unroll 4
+  for (int kt = blockIdx.y * kDqTiles; kt < kt1; ++kt) {
     const int64_t tile = (row / kTileRows) * KT + kt;
     const int64_t k0 = (int64_t)kt * kTileK + lane * 8;
-    int64_t orow = row;
-    if (p.il > 0) {
-      const int64_t j = (row / 128) * 64 + (row % 64);
-      if (j >= p.il) continue;
-      orow = (j / 8) * 16 + (j % 8) + ((row % 128) >= 64 ? 8 : 0);
-    }
     if (k0 >= p.K) continue;
     const uint32_t w =
         __ldg(reinterpret_cast<const uint32_t*>(p.codes + tile * kTileBytes + chunk_off(rr, lane >> 2) + (lane & 3) * 4));
     const uint32_t sb = __ldg(p.scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, NV ? lane >> 1 : lane >> 2));
-    float s = NV ? e4m3_to_f32(sb) * __ldg(p.row_scale + row) : e8m0_to_f32(sb);
+    const float s = NV ? e4m3_to_f32(sb) * rs : e8m0_to_f32(sb);
     uint32_t h[4];
     e2m1x8_to_f16(w, h);
     float v[8];
@@ -260,8 +260,7 @@ static cudaError_t quantize_t(const Fp4QuantArgs& p, cudaStream_t st) {
 
 template <bool NV>
 static cudaError_t dequant_t(const Fp4DequantArgs& p, cudaStream_t st) {
-  const int64_t units = (int64_t)p.R * tiles_k(p.K);
-  const unsigned grid = (unsigned)std::min<int64_t>((units + 7) / 8, 148 * 64);
+  const dim3 grid((unsigned)((p.R + 7) / 8), (tiles_k(p.K) + kDqTiles - 1) / kDqTiles);
   switch (p.out) {
     case 0: fp4_dequant_kernel<NV, 0><<<grid, 256, 0, st>>>(p); break;
     case 1: fp4_dequant_kernel<NV, 1><<<grid, 256, 0, st>>>(p); break;

@@ -92,10 +92,7 @@ def quantize4(x: torch.Tensor, fmt: str = "nvfp4") -> Matrix4:
 
 def dequantize4(m: Matrix4, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """The values of ``m`` as [rows, k] in bf16, f16 or fp32 (``out``: written there, its type)."""
-    if out is None:
-        out = torch.empty(m.rows, m.k, dtype=dtype, device=m.codes.device)
-    _ext.require().fp4_dequantize(m.handle, out)
-    return out
+    return _ext.require().fp4_dequantize(m.handle, out, dtype)
 
 
 def linear4(x: torch.Tensor, w: Matrix4, y: torch.Tensor, mode: int = GEMV_BF16, act4: bool = False) -> torch.Tensor:
