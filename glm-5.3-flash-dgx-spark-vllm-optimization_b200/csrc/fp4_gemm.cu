@@ -4,16 +4,22 @@
 // scale per 32): the tensor core multiplies e2m1 codes, applies both block scales and sums in fp32, at four times the
 // bf16 rate.  Row scales (nvfp4) are applied to the fp32 result.
 //
-// Persistent, one CTA per SM, output tiles of 128 x BN in bands of 8 row blocks.  Both operands are tile images (fp4.cuh),
-// so a K step of 256 is one contiguous cp.async.bulk per 128-row block and array, already swizzled.  Warp roles:
-//   warp 0    producer: fills a 4-stage (BN 256) ring, continuously across tiles
-//   warp 1    allocates TMEM; one thread copies the block scales of the stage to TMEM (tcgen05.cp, executed in order with
-//             the mma of the same thread) and issues the four K = 64 mma of the stage
+// Persistent, one CTA per SM.  Both operands are tile images (fp4.cuh), so a K step of 256 is one contiguous cp.async.bulk
+// per 128-row block and array, already swizzled.  Two forms:
+//   PAIR    256 x 256 tiles by a cluster of two CTAs (cta_group::2): each holds 128 rows of A, half of the tile's rows of W
+//           and all of its scales, so a step brings 38 KB into an SM (nvfp4) where a CTA alone with 128 x 256 needs 54 KB;
+//           (8192 x 24576 x 4096 mxfp4: 390 us, 460 alone)
+//   single  128 x 128 tiles, for fewer tiles than would fill the SMs in pairs
+// Tiles go in bands of 8 row blocks (pairs: 8 pairs).  Warp roles:
+//   warp 0    producer: fills the ring, continuously across tiles
+//   warp 1    allocates TMEM; one thread (of rank 0) copies the block scales of the stage to TMEM (tcgen05.cp, executed in
+//             order with the mma of the same thread) and issues the four K = 64 mma of the stage.  Rank 1's thread passes
+//             on that its stage has landed (a plain arrival: with a cluster-scope release it took 1000 clocks a stage)
 //   warps 2-9 epilogue: tcgen05.ld, row scales, output (four warps, one per scheduler, take longer over the SwiGLU epilogue
 //             than the main loop: 700 us instead of 340 for 8192 x 24576 x 4096)
-// TMEM (512 columns): scales at 448..495; with BN = 256 the two accumulators are columns 0..255 and 192..447.  They share
-// 64 columns, which the epilogue of a tile reads first and then hands back, so the main loop of the next tile waits for
-// a quarter of the epilogue's loads only.
+// TMEM (512 columns): scales at 448..495; a pair's two accumulators are columns 0..255 and 192..447.  They share 64
+// columns, which the epilogue of a tile reads first and then hands back, so the main loop of the next tile waits for a
+// quarter of the epilogue's loads only.
 //
 // GEMV_SWIGLU: W4 is a gate/up image (per 128-row block 64 gate rows, then their 64 up rows); the epilogue forms
 // silu(min(g, L)) * clip(u, -L, L) in fp32 and quantises it in place: a thread holds 32 consecutive activations of one row,
@@ -39,15 +45,19 @@ constexpr int kGemmThreads = 64 + kEpiWarps * 32;
 constexpr int kBandM = 8;
 constexpr uint32_t kSfA = 448, kSfB = 464;            // TMEM columns of the scales
 
-template <bool NV, int BN>
+template <bool NV, bool PAIR>
 struct GemmCfg {
-  static constexpr int kNB = BN / 128;                // 128-row blocks of W per tile
+  static constexpr int kBN = PAIR ? 256 : 128;        // columns of a tile
+  static constexpr int kNB = kBN / 128;               // 128-row blocks of W per tile
   static constexpr int kSB = Fmt<NV>::kScaleBytes;
   static constexpr int kAtoms = kSB / 512;            // scale atoms per block and stage
-  static constexpr int kStage = (1 + kNB) * (kTileBytes + kSB);
-  static constexpr int kStages = BN == 256 ? 4 : 6;
+  // a stage: codes of A, codes of W (one block each), scales of A, scales of W (all of the tile)
+  static constexpr int kOffSA = 2 * kTileBytes, kOffSB = kOffSA + kSB;
+  static constexpr int kStage = kOffSB + kNB * kSB;
+  static constexpr int kStages = (226 * 1024 - 1024) / kStage > 6 ? 6 : (226 * 1024 - 1024) / kStage;
   static constexpr int kSmem = kStages * kStage + 1024;
-  static constexpr uint32_t kBuf = BN == 256 ? 192 : 128;   // column of the second accumulator
+  static constexpr uint32_t kBuf = PAIR ? 192 : 128;  // column of the second accumulator
+  static_assert(kStage % 1024 == 0, "tiles are 1024-byte aligned");
 };
 
 __device__ __forceinline__ void tile_mn(int t, int MT, int NT, int& m, int& n) {
@@ -65,7 +75,7 @@ __device__ __forceinline__ void store32(const Fp4GemmArgs& p, int row, int nb, f
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       if (full) {
-        const float4 t = *reinterpret_cast<const float4*>(p.b_row + nb + i);
+        const float4 t = __ldcg(reinterpret_cast<const float4*>(p.b_row + nb + i));
         v[i] *= rs * t.x; v[i + 1] *= rs * t.y; v[i + 2] *= rs * t.z; v[i + 3] *= rs * t.w;
       } else {
 #pragma unroll
@@ -123,8 +133,8 @@ __device__ __forceinline__ void swiglu32(const Fp4GemmArgs& p, int row, int j0, 
   for (int i = 0; i < 32; i += 4) {
     float4 sg = make_float4(1.f, 1.f, 1.f, 1.f), su = sg;
     if constexpr (NV) {
-      sg = __ldg(reinterpret_cast<const float4*>(p.b_row + r0 + i));
-      su = __ldg(reinterpret_cast<const float4*>(p.b_row + r0 + 64 + i));
+      sg = __ldcg(reinterpret_cast<const float4*>(p.b_row + r0 + i));
+      su = __ldcg(reinterpret_cast<const float4*>(p.b_row + r0 + 64 + i));
     }
     const float gs[4] = {sg.x, sg.y, sg.z, sg.w}, us[4] = {su.x, su.y, su.z, su.w};
 #pragma unroll
@@ -183,10 +193,10 @@ __device__ __forceinline__ void swiglu32(const Fp4GemmArgs& p, int row, int j0, 
       make_uint4(code[0], code[1], code[2], code[3]);
 }
 
-template <bool NV, int BN, bool SWI>
+template <bool NV, bool PAIR, bool SWI>
 __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p) {
-  using C = GemmCfg<NV, BN>;
-  constexpr int kStages = C::kStages;
+  using C = GemmCfg<NV, PAIR>;
+  constexpr int kStages = C::kStages, kG = PAIR ? 2 : 1, BN = C::kBN;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], drain;
@@ -195,55 +205,72 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
   volatile int* fail = &fail_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
   const int KT = tiles_k(p.K);
   const int ksteps = (p.K + 63) / 64;
-  const int MT = (p.M + 127) / 128, NB = (p.N + 127) / 128, NT = (NB + C::kNB - 1) / C::kNB;
+  const int MB = (p.M + 127) / 128, NB = (p.N + 127) / 128;
+  const int MT = (MB + kG - 1) / kG, NT = (NB + C::kNB - 1) / C::kNB;
   const int tiles = MT * NT;
+  const int t0 = (int)blockIdx.x / kG, tstep = (int)gridDim.x / kG;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      tc::bar_init(&full[s], 1);
+      // rank 0 of a pair: its own copies, and word from rank 1 that its have landed
+      tc::bar_init(&full[s], PAIR && rank == 0 ? 2 : 1);
       tc::bar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       tc::bar_init(&tfull[b], 1);
-      tc::bar_init(&tempty[b], kEpiWarps);
+      tc::bar_init(&tempty[b], kG * kEpiWarps);
     }
     tc::bar_init(&drain, 1);
     fail_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tc::tmem_alloc(&tmem_s, 512);
+  if (warp == 1) {
+    if constexpr (PAIR) tmem_alloc_pair(&tmem_s, 512);
+    else tc::tmem_alloc(&tmem_s, 512);
+  }
   tc::fence_before();
   __syncthreads();
+  if constexpr (PAIR) {
+    cluster_arrive();
+    cluster_wait();
+  }
   tc::fence_after();
   const uint32_t tmem = tmem_s;
+  pdl_trigger();
+  pdl_wait();
 
   if (warp == 0) {
     if (elect_one()) {
       uint32_t it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        int mb, nt;
-        tile_mn(t, MT, NT, mb, nt);
-        const int nblk = min(C::kNB, NB - nt * C::kNB);
+      for (int t = t0; t < tiles && ok; t += tstep) {
+        int mt, nt;
+        tile_mn(t, MT, NT, mt, nt);
+        const int mb = mt * kG + rank;                 // this CTA's rows of A
+        const int nb = nt * C::kNB + rank;             // and of W
+        const int nsc = min(C::kNB, NB - nt * C::kNB); // blocks of W that exist
+        const bool has_a = mb < MB, has_b = nb < NB;
+        const uint32_t bytes = (has_a ? kTileBytes + C::kSB : 0) + (has_b ? kTileBytes : 0) + nsc * C::kSB;
         for (int kt = 0; kt < KT; ++kt, ++it) {
           const int s = it % kStages;
           if (it >= kStages && !tc::bar_wait(&empty[s], ((it / kStages) - 1) & 1, fail, &g_gemm_err, 1)) {
             ok = false;
             break;
           }
-          uint8_t* a = smem + s * C::kStage;
-          uint8_t* sa = a + (1 + C::kNB) * kTileBytes;
-          bulk_expect(&full[s], (uint32_t)(1 + nblk) * (kTileBytes + C::kSB));
-          const int64_t ta = (int64_t)mb * KT + kt;
-          bulk_load(a, p.a_codes + ta * kTileBytes, kTileBytes, &full[s]);
-          bulk_load(sa, p.a_scales + ta * C::kSB, C::kSB, &full[s]);
-          for (int b = 0; b < nblk; ++b) {
-            const int64_t tb = (int64_t)(nt * C::kNB + b) * KT + kt;
-            bulk_load(a + (1 + b) * kTileBytes, p.b_codes + tb * kTileBytes, kTileBytes, &full[s]);
-            bulk_load(sa + (1 + b) * C::kSB, p.b_scales + tb * C::kSB, C::kSB, &full[s]);
+          uint8_t* st = smem + s * C::kStage;
+          bulk_expect(&full[s], bytes);
+          if (has_a) {
+            const int64_t ta = (int64_t)mb * KT + kt;
+            bulk_load(st, p.a_codes + ta * kTileBytes, kTileBytes, &full[s]);
+            bulk_load(st + C::kOffSA, p.a_scales + ta * C::kSB, C::kSB, &full[s]);
           }
+          if (has_b) bulk_load(st + kTileBytes, p.b_codes + ((int64_t)nb * KT + kt) * kTileBytes, kTileBytes, &full[s]);
+          for (int b = 0; b < nsc; ++b)
+            bulk_load(st + C::kOffSB + b * C::kSB, p.b_scales + ((int64_t)(nt * C::kNB + b) * KT + kt) * C::kSB, C::kSB,
+                      &full[s]);
         }
       }
       if (*fail) {
@@ -257,11 +284,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
     if (elect_one()) {
       uint32_t it = 0, tl = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++tl) {
+      for (int t = t0; t < tiles && ok; t += tstep, ++tl) {
+        if (PAIR && rank == 1) {
+          for (int kt = 0; kt < KT; ++kt, ++it) {
+            const int s = it % kStages;
+            if (!tc::bar_wait(&full[s], (it / kStages) & 1, fail, &g_gemm_err, 5)) { ok = false; break; }
+            signal_at(&full[s], 0);
+          }
+          continue;
+        }
         const uint32_t buf = tl & 1;
-        // BN 256: the shared columns of the tile before; BN 128: the buffer's last tile
-        const uint32_t lag = BN == 256 ? 1 : 2;
-        if (tl >= lag && !tc::bar_wait(&tempty[(tl - lag) & 1], ((tl - lag) >> 1) & 1, fail, &g_gemm_err, 4)) break;
+        // pairs: the shared columns of the tile before; single: the buffer's last tile
+        const uint32_t lag = PAIR ? 1 : 2;
+        if (tl >= lag &&
+            !tc::bar_wait(&tempty[(tl - lag) & 1], ((tl - lag) >> 1) & 1, fail, &g_gemm_err, 4)) break;
         tc::fence_after();
         const uint32_t d = tmem + buf * C::kBuf;
         for (int kt = 0; kt < KT; ++kt, ++it) {
@@ -271,15 +307,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
             break;
           }
           tc::fence_after();
-          const uint32_t a = tc::saddr(smem + s * C::kStage);
-          const uint32_t b = a + kTileBytes;
-          const uint32_t sa = a + (1 + C::kNB) * kTileBytes;
+          const uint32_t a = tc::saddr(smem + s * C::kStage), b = a + kTileBytes;
 #pragma unroll
           for (int at = 0; at < C::kAtoms; ++at) {
-            copy_scales(tmem + kSfA + at * 4, sa + at * 512);
+            copy_scales<kG>(tmem + kSfA + at * 4, a + C::kOffSA + at * 512);
 #pragma unroll
             for (int nb = 0; nb < C::kNB; ++nb)
-              copy_scales(tmem + kSfB + at * (4 * C::kNB) + nb * 4, sa + (1 + nb) * C::kSB + at * 512);
+              copy_scales<kG>(tmem + kSfB + at * (4 * C::kNB) + nb * 4, a + C::kOffSB + nb * C::kSB + at * 512);
           }
           const int n = min(4, ksteps - kt * 4);
 #pragma unroll
@@ -287,16 +321,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
             if (k >= n) break;
             const int at = NV ? k : k >> 1;
             const uint32_t sf = NV ? 0u : (uint32_t)(k & 1) * 2;
-            mma4<NV>(d, tc::desc_sw128(a + k * 32), tc::desc_sw128(b + k * 32), idesc4(128, BN, !NV, sf),
-                     tmem + kSfA + at * 4, tmem + kSfB + at * (4 * C::kNB), (kt > 0 || k > 0) ? 1u : 0u);
+            mma4<NV, kG>(d, tc::desc_sw128(a + k * 32), tc::desc_sw128(b + k * 32), idesc4(128 * kG, BN, !NV, sf),
+                         tmem + kSfA + at * 4, tmem + kSfB + at * (4 * C::kNB), (kt > 0 || k > 0) ? 1u : 0u);
           }
-          tc::commit(&empty[s]);
+          if constexpr (PAIR) commit_pair(&empty[s]);
+          else tc::commit(&empty[s]);
         }
-        if (ok) tc::commit(&tfull[buf]);
+        if (ok) {
+          if constexpr (PAIR) commit_pair(&tfull[buf]);
+          else tc::commit(&tfull[buf]);
+        }
       }
-      if (*fail) {
+      if (*fail && rank == 0) {
         int none = 0;
-        tc::commit(&drain);
+        if constexpr (PAIR) commit_pair(&drain);
+        else tc::commit(&drain);
         tc::bar_wait(&drain, 0, &none, nullptr, 0);
       }
     }
@@ -306,25 +345,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
     // tempty says that those are read; that of part 1, that it is done with the tile before
     const int quad = warp & 3, part = (warp - 2) >> 2;
     uint32_t tl = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++tl) {
+    for (int t = t0; t < tiles; t += tstep, ++tl) {
       const uint32_t buf = tl & 1;
-      int mb, nt;
-      tile_mn(t, MT, NT, mb, nt);
+      int mt, nt;
+      tile_mn(t, MT, NT, mt, nt);
       if (!tc::warp_wait(&tfull[buf], (tl >> 1) & 1, fail, &g_gemm_err, 3)) break;
       tc::fence_after();
-      const int row = mb * 128 + quad * 32 + lane;
+      const int row = (mt * kG + rank) * 128 + quad * 32 + lane;
       const bool live = row < p.M;
       const float rs = p.a_row && live ? p.a_row[row] : p.a_const;
       const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + buf * C::kBuf;
       auto release = [&]() {
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) tc::bar_arrive(&tempty[buf]);
+        if (lane == 0) {
+          if (PAIR && rank == 1) signal_at(&tempty[buf], 0);
+          else tc::bar_arrive(&tempty[buf]);
+        }
       };
-      if (BN == 256 && part == 1) release();
+      if (PAIR && part == 1) release();
       if constexpr (SWI) {
         const int wide = ((p.width + 63) / 64) * 64;
-        if constexpr (BN == 256) {
+        if constexpr (PAIR) {
           // a block (64 gate, 64 up columns) per part.  The shared columns are the up half of block 1 (buffer 0) or the gate
           // half of block 0 (buffer 1)
           const int blk = buf == 0 ? 1 - part : part;
@@ -357,12 +399,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
         constexpr int kUnits = BN / 128;              // units of 64 columns per part
 #pragma unroll 1
         for (int i = 0; i < kUnits; ++i) {
-          // buffer 0 of BN 256: units 3, 2 and 0, 1
-          const int u = BN == 256 && buf == 0 ? (part == 0 ? 3 - i : i) : part * kUnits + i;
+          // buffer 0 of a pair: units 3, 2 and 0, 1
+          const int u = PAIR && buf == 0 ? (part == 0 ? 3 - i : i) : part * kUnits + i;
           float x0[32], x1[32];
           tc::tmem_ld32(base + u * 64, x0);
           tc::tmem_ld32(base + u * 64 + 32, x1);
-          if (BN == 256 ? part == 0 && i == 0 : true) release();
+          if (PAIR ? part == 0 && i == 0 : true) release();
           if (live && n0 + u * 64 < p.N) store32(p, row, n0 + u * 64, rs, x0);
           if (live && n0 + u * 64 + 32 < p.N) store32(p, row, n0 + u * 64 + 32, rs, x1);
         }
@@ -371,9 +413,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
   }
   tc::fence_before();
   __syncthreads();
+  if constexpr (PAIR) {
+    // rank 0's mma read rank 1's shared memory and write its TMEM; rank 1 arrives on rank 0's barriers
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     tc::fence_after();
-    tc::tmem_free(tmem, 512);
+    if constexpr (PAIR) tmem_free_pair(tmem, 512);
+    else tc::tmem_free(tmem, 512);
   }
 }
 
@@ -388,27 +436,48 @@ static cudaError_t sm_count(int dev, int* out) {
   return e;
 }
 
-template <bool NV, int BN, bool SWI>
+template <bool NV, bool PAIR, bool SWI>
 static cudaError_t launch_gemm(const Fp4GemmArgs& p, int dev, int sms, cudaStream_t st) {
-  using C = GemmCfg<NV, BN>;
-  auto kern = fp4_gemm_kernel<NV, BN, SWI>;
+  using C = GemmCfg<NV, PAIR>;
+  auto kern = fp4_gemm_kernel<NV, PAIR, SWI>;
   static std::atomic<bool> ready[kMaxDev];            // the shared memory limit, raised once per device
   if (dev >= kMaxDev || !ready[dev].load(std::memory_order_relaxed)) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;
     if (dev < kMaxDev) ready[dev].store(true, std::memory_order_relaxed);
   }
-  const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + BN - 1) / BN);
-  kern<<<(unsigned)std::min<int64_t>(tiles, sms), kGemmThreads, C::kSmem, st>>>(p);
-  return cudaGetLastError();
+  constexpr int kG = PAIR ? 2 : 1;
+  const int64_t tiles = (((int64_t)p.M + 128 * kG - 1) / (128 * kG)) * (((int64_t)p.N + C::kBN - 1) / C::kBN);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles, sms / kG) * kG);
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int na = 0;
+  if (PAIR) {
+    at[na].id = cudaLaunchAttributeClusterDimension;
+    at[na].val.clusterDim.x = 2;
+    at[na].val.clusterDim.y = 1;
+    at[na].val.clusterDim.z = 1;
+    ++na;
+  }
+  if (g53_pdl_on()) {
+    at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = na;
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 template <bool NV>
 static cudaError_t gemm_t(const Fp4GemmArgs& p, int dev, int sms, cudaStream_t st) {
-  const bool wide = (int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256) >= sms;
+  const bool pair = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) >= sms / 2;
   if (p.mode == GEMV_SWIGLU)
-    return wide ? launch_gemm<NV, 256, true>(p, dev, sms, st) : launch_gemm<NV, 128, true>(p, dev, sms, st);
-  return wide ? launch_gemm<NV, 256, false>(p, dev, sms, st) : launch_gemm<NV, 128, false>(p, dev, sms, st);
+    return pair ? launch_gemm<NV, true, true>(p, dev, sms, st) : launch_gemm<NV, false, true>(p, dev, sms, st);
+  return pair ? launch_gemm<NV, true, false>(p, dev, sms, st) : launch_gemm<NV, false, false>(p, dev, sms, st);
 }
 
 }  // namespace fp4

@@ -4,6 +4,7 @@
 // fp4_quantize: per block a maximum of magnitudes, a scale from it, 16 codes per thread.  The row (nvfp4 needs its
 // maximum first) stays in registers between the two uses, so the input is read once.  Both kernels move 2 + 1/2 + 1/16
 // (1/32) bytes per element and are bound by HBM.
+// Launched programmatically, so what earlier kernels wrote is read from L2 (__ldcg), not through the read-only path.
 // Infinities and NaN: an mxfp4 block that holds one reads back as NaN, an nvfp4 row that holds one likewise (its row
 // scale is NaN).  Magnitudes are compared as integers, so a NaN counts as the largest.
 #include <algorithm>
@@ -39,17 +40,20 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(Fp4QuantArgs p) {
   const int nb = KT * 16;                            // blocks of 16, padding included
   const int nk = (int)(p.K / 16);
   const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + (live ? row : 0) * p.ldx;
+  pdl_trigger();
+  pdl_wait();
 
   auto load = [&](int b, uint32_t (&w)[8]) {
     if (live && b < nk) {
       if (p.vec) {
-        const uint4 a = ldg_nc_v4(x + (int64_t)b * 16), c = ldg_nc_v4(x + (int64_t)b * 16 + 8);
+        const uint4* v = reinterpret_cast<const uint4*>(x + (int64_t)b * 16);
+        const uint4 a = __ldcg(v), c = __ldcg(v + 1);
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
         w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          w[i] = (uint32_t)__ldg(x + (int64_t)b * 16 + 2 * i) | ((uint32_t)__ldg(x + (int64_t)b * 16 + 2 * i + 1) << 16);
+          w[i] = (uint32_t)__ldcg(x + (int64_t)b * 16 + 2 * i) | ((uint32_t)__ldcg(x + (int64_t)b * 16 + 2 * i + 1) << 16);
       }
     } else {
 #pragma unroll
@@ -177,6 +181,8 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(Fp4DequantArgs p) {
   const int KT = tiles_k(p.K);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = (int64_t)blockIdx.x * 8 + warp;
+  pdl_trigger();
+  pdl_wait();
   if (row >= p.R) return;
   const int rr = (int)(row % kTileRows);
   int64_t orow = row;
@@ -185,7 +191,7 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(Fp4DequantArgs p) {
     if (j >= p.il) return;
     orow = (j / 8) * 16 + (j % 8) + ((row % 128) >= 64 ? 8 : 0);
   }
-  const float rs = NV ? __ldg(p.row_scale + row) : 1.f;
+  const float rs = NV ? __ldcg(p.row_scale + row) : 1.f;
   const int kt1 = min(KT, ((int)blockIdx.y + 1) * kDqTiles);
 #pragma unroll 4
   for (int kt = blockIdx.y * kDqTiles; kt < kt1; ++kt) {
@@ -193,8 +199,8 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(Fp4DequantArgs p) {
     const int64_t k0 = (int64_t)kt * kTileK + lane * 8;
     if (k0 >= p.K) continue;
     const uint32_t w =
-        __ldg(reinterpret_cast<const uint32_t*>(p.codes + tile * kTileBytes + chunk_off(rr, lane >> 2) + (lane & 3) * 4));
-    const uint32_t sb = __ldg(p.scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, NV ? lane >> 1 : lane >> 2));
+        __ldcg(reinterpret_cast<const uint32_t*>(p.codes + tile * kTileBytes + chunk_off(rr, lane >> 2) + (lane & 3) * 4));
+    const uint32_t sb = __ldcg(p.scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, NV ? lane >> 1 : lane >> 2));
     const float s = NV ? e4m3_to_f32(sb) * rs : e8m0_to_f32(sb);
     uint32_t h[4];
     e2m1x8_to_f16(w, h);
@@ -243,9 +249,8 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(Fp4DequantArgs p) {
 template <bool NV, bool F16, int T, int B, bool REREAD>
 static cudaError_t launch_q(const Fp4QuantArgs& p, cudaStream_t st) {
   constexpr int kRows = 256 / T;
-  fp4_quantize_kernel<NV, F16, T, B, REREAD><<<(unsigned)((p.R + kRows - 1) / kRows), 256, 0, st>>>(p);
-  G53_CHECK_LAUNCH();
-  return cudaSuccess;
+  return g53_launch_pdl(fp4_quantize_kernel<NV, F16, T, B, REREAD>, dim3((unsigned)((p.R + kRows - 1) / kRows)), dim3(256),
+                        0, st, 1, p);
 }
 
 template <bool NV, bool F16>
@@ -262,12 +267,10 @@ template <bool NV>
 static cudaError_t dequant_t(const Fp4DequantArgs& p, cudaStream_t st) {
   const dim3 grid((unsigned)((p.R + 7) / 8), (tiles_k(p.K) + kDqTiles - 1) / kDqTiles);
   switch (p.out) {
-    case 0: fp4_dequant_kernel<NV, 0><<<grid, 256, 0, st>>>(p); break;
-    case 1: fp4_dequant_kernel<NV, 1><<<grid, 256, 0, st>>>(p); break;
-    default: fp4_dequant_kernel<NV, 2><<<grid, 256, 0, st>>>(p); break;
+    case 0: return g53_launch_pdl(fp4_dequant_kernel<NV, 0>, grid, dim3(256), 0, st, 1, p);
+    case 1: return g53_launch_pdl(fp4_dequant_kernel<NV, 1>, grid, dim3(256), 0, st, 1, p);
+    default: return g53_launch_pdl(fp4_dequant_kernel<NV, 2>, grid, dim3(256), 0, st, 1, p);
   }
-  G53_CHECK_LAUNCH();
-  return cudaSuccess;
 }
 
 }  // namespace fp4

@@ -209,28 +209,10 @@ __device__ __forceinline__ bool sk_wait(uint64_t* b, uint32_t ph, volatile int* 
   }
   return true;
 }
-// wait on a barrier that other CTAs of the cluster arrive on, with cluster-scope acquire
-__device__ __forceinline__ bool sk_wait_cluster(uint64_t* b, uint32_t ph, volatile int* stop) {
-  for (uint32_t n = 0;; ++n) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0,1,0,p;\n}\n" : "=r"(ok) : "r"(tc::saddr(b)), "r"(ph) : "memory");
-    if (ok) return true;
-    if (*stop) return false;
-    if (n > (1u << 22)) {
-      *stop = 1;
-      atomicExch(&g_skinny_err, kErrSk + 1);
-      return false;
-    }
-  }
-}
 __device__ __forceinline__ void sk_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }   // the epilogue warps
 __device__ __forceinline__ void sk_prefetch(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // WIDE: mma N up to 256 (17..32 rows), one CTA per SM; otherwise N <= 128 and two CTAs per SM
 template <bool NV, bool WIDE, bool INLINE>
@@ -432,8 +414,8 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       float rs0 = 1.f, rs1 = 1.f;
       if (NV && f_grp < groups) {
         const int n = nb * 128 + j_lo + f_row;
-        if (n < p.N) rs0 = __ldg(p.row_scale + n);
-        if (n + 64 < p.N) rs1 = __ldg(p.row_scale + n + 64);
+        if (n < p.N) rs0 = __ldcg(p.row_scale + n);
+        if (n + 64 < p.N) rs1 = __ldcg(p.row_scale + n + 64);
       }
       if (!dead) {
         int ok = 0;
@@ -468,14 +450,11 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
         if (warp == 2 && lane < CL && lane != rank) {
           // cluster-scope release: the CTA's stores, seen through the barrier above, come before the arrival
           asm volatile("fence.acq_rel.cluster;" ::: "memory");
-          uint32_t remote;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote)
-                       : "r"(tc::saddr(&recv_bar[blk & 1])), "r"(lane));
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+          arrive_at(&recv_bar[blk & 1], lane);
         }
         __syncwarp();
         if (!dead) {
-          const bool ok = sk_wait_cluster(&recv_bar[blk & 1], (blk >> 1) & 1, stop);
+          const bool ok = bar_wait_cluster(&recv_bar[blk & 1], (blk >> 1) & 1, stop, &g_skinny_err, kErrSk + 1);
           dead = !__all_sync(0xffffffffu, ok);
         }
       }

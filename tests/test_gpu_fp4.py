@@ -240,7 +240,7 @@ def test_linear_exact_activations_above_16_rows(fmt, m):
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,n,k", [(17, 8, 32), (64, 128, 64), (100, 100, 96), (128, 256, 256), (129, 257, 288),
                                    (300, 1000, 1536), (70, 130, 4128), (1000, 520, 320), (2500, 4100, 544),
-                                   (4096, 2048, 1024)])
+                                   (4096, 2048, 1024), (2433, 2817, 96), (129, 19100, 288)])
 def test_linear_4bit_activations(fmt, m, n, k):
     x, w = acts(m, k, m), weight(n, k, n)
     w4 = fp4.quantize4(w, fmt)
@@ -334,7 +334,7 @@ def test_mlp_exact_activations(fmt, m, k, width, n):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,k,width,n", [(17, 256, 32, 8), (40, 512, 96, 40), (130, 288, 160, 200), (257, 1024, 1536, 300),
-                                         (2500, 320, 4128, 264)])
+                                         (2500, 320, 4128, 264), (2433, 96, 1376, 64)])
 def test_mlp_4bit_activations(fmt, m, k, width, n):
     limit = 2.0
     x, gate, up, down = acts(m, k, m), weight(width, k, 1), weight(width, k, 2), weight(n, width, 3)
