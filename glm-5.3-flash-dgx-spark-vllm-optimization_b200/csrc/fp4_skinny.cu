@@ -20,22 +20,22 @@
 //
 // fp4_skinny: a CTA takes a 128-row block of W and a slice of its K tiles; a cluster of CL CTAs shares a block, and
 // clusters walk the blocks.  Warp 0 streams tiles into a ring (contiguous cp.async.bulk), warp 1 copies the scales to TMEM
-// and issues the mma, warps 2-5 (form the expansion,) read the sums (a thread holds one weight row), send them to the rank
-// of the cluster that owns the row (distributed shared memory, one arrival per sender) and finish the rows they own, adding
-// in rank order: the result does not depend on timing.  Two receive buffers alternate: a rank can only send block b + 2
-// after it received every rank's b + 1, which each sent after it had finished reading b.
+// and issues the mma, warps 2-9 (form the expansion,) read the sums (a thread holds one weight row), send them to the rank
+// of the cluster that owns the row (st.async into its shared memory, counted in bytes on its barrier: stores with a
+// cluster-scope release behind them took a microsecond) and finish the rows they own, adding in rank order: the result does
+// not depend on timing.  Two receive buffers alternate: a rank can only send block b + 2 after it received every rank's b +
+// 1, which each sent after it had finished reading b.  No barrier is needed at the end: a CTA leaves after it has received
+// all that is sent to it.
 //
 // Before griddepcontrol.wait only prefetches into L2 are issued: the weights may be what the previous kernel writes.
-// Waits are bounded; one that runs out sets the error word and the CTA goes on without waiting, so every barrier is
-// still reached, copies and mma in flight are waited for (bounded) and the TMEM is freed.
+// Waits are bounded; one that runs out sets the error word, and the CTA goes on without the main loop's waits but sends and
+// receives all the same, so that no CTA of the cluster is left waiting or written to after it has gone; copies and mma in
+// flight are waited for (bounded) and the TMEM is freed.
 #include <algorithm>
 #include <atomic>
-#include <cooperative_groups.h>
 #include "fp4.cuh"
 #include "fp4_tc.cuh"
 #include "launchers.h"
-
-namespace cg = cooperative_groups;
 
 namespace g53 {
 namespace fp4 {
@@ -43,7 +43,7 @@ namespace fp4 {
 __device__ int g_skinny_err = 0;
 
 constexpr int kTerms = 8;
-constexpr int kEpi = 4;                               // warps of the expansion and the epilogue
+constexpr int kEpi = 8;                               // warps of the expansion and the epilogue
 constexpr int kSkThreads = 64 + kEpi * 32;
 constexpr int kErrSk = 0x6b40;
 
@@ -209,9 +209,31 @@ __device__ __forceinline__ bool sk_wait(uint64_t* b, uint32_t ph, volatile int* 
   }
   return true;
 }
-__device__ __forceinline__ void sk_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }   // the epilogue warps
+__device__ __forceinline__ void sk_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }   // the epilogue warps
 __device__ __forceinline__ void sk_prefetch(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
+// one output of the modes that write sums
+__device__ __forceinline__ void store1(const Fp4SkinnyArgs& p, int tok, int n, float v) {
+  const int64_t off = (int64_t)tok * p.ldy + n;
+  if (p.mode == GEMV_BF16) {
+    reinterpret_cast<__nv_bfloat16*>(p.y)[off] = f2bf(v);
+  } else {
+    float* y = reinterpret_cast<float*>(p.y) + off;
+    *y = p.mode == GEMV_F32_ACC ? *y + v : v;
+  }
+}
+// four values into the shared memory of a CTA of the cluster, counted on its barrier (both addresses mapped to that CTA)
+__device__ __forceinline__ void send4(uint32_t dst, uint32_t bar, const float (&v)[4]) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(dst), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+               "r"(__float_as_uint(v[3])), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
 }
 
 // WIDE: mma N up to 256 (17..32 rows), one CTA per SM; otherwise N <= 128 and two CTAs per SM
@@ -225,12 +247,12 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[8], empty[8], recv_bar[2], tfull, tempty, xready, drain;
   __shared__ uint32_t tmem_s, xmax[32];
-  __shared__ float xfac[32];
+  __shared__ float xfac[32 + 4];                      // read four at a time
   __shared__ int stop_s;
   volatile int* stop = &stop_s;
   uint8_t* xs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = xs + (INLINE ? pl.xbytes : 0);
-  float* recv = reinterpret_cast<float*>(ring + pl.stages * pl.stage_bytes);   // [2][CL][M][2][j_per]
+  float* recv = reinterpret_cast<float*>(ring + pl.stages * pl.stage_bytes);   // [2][CL][2][j_per][Mp]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int CL = pl.CL;
@@ -250,8 +272,8 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       tc::bar_init(&full[s], 1);
       tc::bar_init(&empty[s], 1);
     }
-    tc::bar_init(&recv_bar[0], CL > 1 ? CL - 1 : 1);
-    tc::bar_init(&recv_bar[1], CL > 1 ? CL - 1 : 1);
+    tc::bar_init(&recv_bar[0], 1);
+    tc::bar_init(&recv_bar[1], 1);
     tc::bar_init(&tfull, 1);
     tc::bar_init(&tempty, kEpi);
     tc::bar_init(&xready, kEpi);
@@ -263,7 +285,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
   if (warp == 1) tc::tmem_alloc(&tmem_s, kCols);
   tc::fence_before();
   __syncthreads();
-  // the peers' barriers are first touched by the epilogue, which waits there
+  // the peers' barriers are first touched by the epilogue, which waits there (mbarrier_init above is the release)
   if (CL > 1) cluster_arrive();
   tc::fence_after();
   const uint32_t tmem = tmem_s;
@@ -307,10 +329,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       }
     }
     __syncwarp();
-    if (CL > 1) {
-      cluster_wait();
-      cluster_arrive();
-    }
+    if (CL > 1) cluster_wait();
   } else if (warp == 1) {
     if (elect_one()) {
       const int ksteps = (p.K + 63) / 64;
@@ -352,20 +371,16 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       }
     }
     __syncwarp();
-    if (CL > 1) {
-      cluster_wait();
-      cluster_arrive();
-    }
+    if (CL > 1) cluster_wait();
   } else {
     const int quad = warp & 3, et = threadIdx.x - 64, part = (warp - 2) >> 2;
     const int r = quad * 32 + lane;                   // row of the block
     const int j = r & 63, half = r >> 6;
     const int owner = j / j_per, jl = j - owner * j_per;
-    const int buf_floats = CL * p.M * 2 * j_per;
-    // finishing: this thread's row pair and its group's first (token, half)
-    const int groups = kEpi * 32 / rows;
-    const int f_row = et % rows, f_grp = et / rows;   // f_grp >= groups: no part in it
+    const int Mp = (p.M + 3) & ~3;
+    const int buf_floats = CL * 2 * j_per * Mp;
     const bool swi = p.mode == GEMV_SWIGLU;
+    const bool direct = CL == 1 && !swi;              // rows finished where they are read
     pdl_wait();
     if constexpr (INLINE) {
       // a thread per block of 16 of the slice (the plan sees to it that there are no more than threads)
@@ -410,95 +425,94 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
     uint32_t blk = 0;
     bool dead = false;
     for (int nb = cid; nb < pl.blocks; nb += pl.clusters, ++blk) {
-      // scales of the rows this thread will finish: loaded under the main loop
-      float rs0 = 1.f, rs1 = 1.f;
-      if (NV && f_grp < groups) {
-        const int n = nb * 128 + j_lo + f_row;
-        if (n < p.N) rs0 = __ldcg(p.row_scale + n);
-        if (n + 64 < p.N) rs1 = __ldcg(p.row_scale + n + 64);
-      }
+      const uint32_t rbar = tc::saddr(&recv_bar[blk & 1]);
+      if (CL > 1 && et == 0) bulk_expect(&recv_bar[blk & 1], (uint32_t)((CL - 1) * 2 * rows * Mp * 4));
+      // scale of this thread's row: loaded under the main loop
+      float rs = 1.f;
+      if (NV && direct && nb * 128 + r < p.N) rs = __ldcg(p.row_scale + nb * 128 + r);
       if (!dead) {
         int ok = 0;
         if (lane == 0) ok = sk_wait(&tfull, blk & 1, stop) ? 1 : 0;
         dead = __shfl_sync(0xffffffffu, ok, 0) == 0;
       }
+      tc::fence_after();
       float* rb = recv + (blk & 1) * buf_floats;
-      // this rank's sums of row r, token tok -> [rank][tok][half][jl] of the owner
-      float* dst = rb + ((int64_t)rank * p.M * 2 + half) * j_per + jl;
-      if (CL > 1 && owner != rank) dst = cg::this_cluster().map_shared_rank(dst, owner);
-      if (!dead) {
-        tc::fence_after();
-        for (int m0 = part * 4; m0 < p.M; m0 += kEpi) {
-          float v[32];
-          tc::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + m0 * kTerms, v);
+      // this rank's sums of row r -> [rank][half][jl][token] of the owner
+      float* dst = rb + ((rank * 2 + half) * j_per + jl) * Mp;
+      const uint32_t rdst = CL > 1 ? map_to(tc::saddr(dst), owner) : 0, rdbar = CL > 1 ? map_to(rbar, owner) : 0;
+      for (int m0 = part * 4; m0 < p.M; m0 += kEpi) {
+        float v[32];
+        if (!dead) tc::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + m0 * kTerms, v);
+        float sum[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sum[i] = 0.f;
+#pragma unroll
+          for (int t = kTerms - 1; t >= 0; --t)       // small terms first
+            sum[i] = NV ? fmaf(v[i * kTerms + t], 1.f / (float)(1 << (3 * t)), sum[i]) : sum[i] + v[i * kTerms + t];
+          if (NV) sum[i] *= xfac[m0 + i];             // rows past M: never used
+        }
+        if (direct) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (m0 + i < p.M && nb * 128 + r < p.N) store1(p, m0 + i, nb * 128 + r, sum[i] * rs);
+        } else if (owner == rank) {
+          *reinterpret_cast<float4*>(dst + m0) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        } else {
+          send4(rdst + m0 * 4, rdbar, sum);
+        }
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) tc::bar_arrive(&tempty);
+      if (direct) continue;
+      sk_sync();                                      // this CTA's own rows
+      if (CL > 1) {
+        const bool ok = bar_wait_cluster(&recv_bar[blk & 1], (blk >> 1) & 1, nullptr, &g_skinny_err, kErrSk + 1);
+        if (!ok) *stop = 1;                           // (waited for in a stopped CTA, too)
+      }
+      // ---- finish rows j_lo.. and + 64, four tokens at a time: consecutive threads on consecutive rows
+      const int units = rows * (Mp / 4) * (swi ? 1 : 2);
+      for (int e = et; e < units; e += kEpi * 32) {
+        const int q = e / rows, row = e - q * rows;
+        const int tok = (swi ? q : q >> 1) * 4, hf = swi ? 0 : q & 1;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
+        for (int c = 0; c < CL; ++c) {
+          const float* src = rb + ((c * 2 + hf) * j_per + row) * Mp + tok;
+          const float4 a = *reinterpret_cast<const float4*>(src);
+          v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+          if (swi) {
+            const float4 b = *reinterpret_cast<const float4*>(src + j_per * Mp);
+            u.x += b.x; u.y += b.y; u.z += b.z; u.w += b.w;
+          }
+        }
+        const int n = nb * 128 + j_lo + row + hf * 64;
+        float vs[4] = {v.x, v.y, v.z, v.w};
+        const float us[4] = {u.x, u.y, u.z, u.w};
+        if (swi) {
+          const int col = nb * 64 + j_lo + row;
+          if (col >= p.width) continue;
+          const float sg = NV ? __ldcg(p.row_scale + n) : 1.f, su = NV ? __ldcg(p.row_scale + n + 64) : 1.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (m0 + i >= p.M) break;
-            float sum = 0.f;
-#pragma unroll
-            for (int t = kTerms - 1; t >= 0; --t)     // small terms first
-              sum = NV ? fmaf(v[i * kTerms + t], 1.f / (float)(1 << (3 * t)), sum) : sum + v[i * kTerms + t];
-            dst[(m0 + i) * 2 * j_per] = NV ? sum * xfac[m0 + i] : sum;
-          }
-        }
-        tc::fence_before();
-      }
-      __syncwarp();
-      if (lane == 0 && !dead) tc::bar_arrive(&tempty);
-      sk_sync();                                      // every row of this CTA is on its way
-      if (CL > 1) {
-        if (warp == 2 && lane < CL && lane != rank) {
-          // cluster-scope release: the CTA's stores, seen through the barrier above, come before the arrival
-          asm volatile("fence.acq_rel.cluster;" ::: "memory");
-          arrive_at(&recv_bar[blk & 1], lane);
-        }
-        __syncwarp();
-        if (!dead) {
-          const bool ok = bar_wait_cluster(&recv_bar[blk & 1], (blk >> 1) & 1, stop, &g_skinny_err, kErrSk + 1);
-          dead = !__all_sync(0xffffffffu, ok);
-        }
-      }
-      // ---- finish rows j_lo.. and + 64: consecutive threads on consecutive rows
-      if (f_grp < groups) {
-        const int halves = swi ? 1 : 2;
-        for (int q = f_grp; q < p.M * halves; q += groups) {
-          const int tok = swi ? q : q >> 1, hf = swi ? 0 : q & 1;
-          float v = 0.f, u = 0.f;
-          for (int c = 0; c < CL; ++c) {
-            const float* src = rb + ((c * p.M + tok) * 2 + hf) * j_per + f_row;
-            v += src[0];
-            if (swi) u += src[j_per];
-          }
-          if (swi) {
-            const int col = nb * 64 + j_lo + f_row;
-            if (col >= p.width) continue;
-            v *= rs0;
-            u *= rs1;
+            if (tok + i >= p.M) break;
+            float g = vs[i] * sg, w = us[i] * su;
             // written so that a NaN stays one
-            v = v > p.limit ? p.limit : v;
-            u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
-            reinterpret_cast<__nv_bfloat16*>(p.y)[(int64_t)tok * p.ldy + col] = f2bf(siluf_(v) * u);
-          } else {
-            const int n = nb * 128 + j_lo + f_row + hf * 64;
-            if (n >= p.N) continue;
-            v *= hf ? rs1 : rs0;
-            const int64_t off = (int64_t)tok * p.ldy + n;
-            if (p.mode == GEMV_BF16) {
-              reinterpret_cast<__nv_bfloat16*>(p.y)[off] = f2bf(v);
-            } else {
-              float* y = reinterpret_cast<float*>(p.y) + off;
-              *y = p.mode == GEMV_F32_ACC ? *y + v : v;
-            }
+            g = g > p.limit ? p.limit : g;
+            w = w > p.limit ? p.limit : w < -p.limit ? -p.limit : w;
+            reinterpret_cast<__nv_bfloat16*>(p.y)[(int64_t)(tok + i) * p.ldy + col] = f2bf(siluf_(g) * w);
           }
+        } else {
+          if (n >= p.N) continue;
+          const float sc = NV ? __ldcg(p.row_scale + n) : 1.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (tok + i < p.M) store1(p, tok + i, n, vs[i] * sc);
         }
       }
     }
-    __syncwarp();
-    if (CL > 1) cluster_arrive();
   }
   tc::fence_before();
-  // no CTA leaves while another of its cluster may still write to it
-  if (CL > 1) cluster_wait();
   __syncthreads();
   if (warp == 1) {
     tc::fence_after();
@@ -508,7 +522,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
 
 constexpr int kMaxDev = 64;
 
-static int sk_recv_bytes(int CL, int M) { return 2 * CL * M * 2 * ((64 + CL - 1) / CL) * 4; }
+static int sk_recv_bytes(int CL, int M) { return 2 * CL * ((M + 3) & ~3) * 2 * ((64 + CL - 1) / CL) * 4; }
 static int sk_budget(bool wide) { return (wide ? 225 : 111) * 1024; }
 
 // Stands in for the product in the question below: the runtime answers one CTA per SM for any kernel that uses TMEM
@@ -578,7 +592,7 @@ static cudaError_t sk_plan(int M, int64_t N, int K, int dev, SkPlan& b, double& 
     if (cl > 1) active -= active / 8;
     const int xbytes = INLINE ? (per * xtile + 1023) / 1024 * 1024 : 0;
     const int stages = std::min(8, (sk_budget(WIDE) - 1024 - xbytes - sk_recv_bytes(cl, M)) / b.stage_bytes);
-    if (stages < 2) continue;
+    if (stages < (INLINE ? 4 : 2)) continue;           // a resident expansion must leave the ring its depth
     const int clusters = std::min(b.blocks, active), rounds = (b.blocks + clusters - 1) / clusters;
     const double c = rounds * per + (rounds - 1) * (4 + 0.08 * M * cl) + 0.047 * M * cl;
     if (b.CL == 0 || c < cost) {

@@ -75,20 +75,14 @@ __device__ __forceinline__ void tmem_free_pair(uint32_t base, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
 }
 // ---- barriers of a cluster
-// arrival on the barrier of a CTA of the cluster, releasing at cluster scope
-__device__ __forceinline__ void arrive_at(uint64_t* b, uint32_t rank) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(tc::saddr(b)), "r"(rank));
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
-}
-// the same where the arriving thread has written nothing itself (it passes on what a barrier told it): a cluster-scope
-// release would cost it about 1000 clocks
+// arrival on the barrier of a CTA of the cluster by a thread that has written nothing itself (it passes on what a barrier
+// told it): a cluster-scope release would cost it about 1000 clocks
 __device__ __forceinline__ void signal_at(uint64_t* b, uint32_t rank) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(tc::saddr(b)), "r"(rank));
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
-// tc::bar_wait with cluster-scope acquire, for barriers that another CTA arrives on
+// tc::bar_wait with cluster-scope acquire, for barriers that another CTA arrives on (fail null: never cut short)
 __device__ __forceinline__ bool bar_wait_cluster(uint64_t* b, uint32_t ph, volatile int* fail, int* err, int code) {
   for (uint32_t n = 0;; ++n) {
     uint32_t ok;
@@ -96,15 +90,16 @@ __device__ __forceinline__ bool bar_wait_cluster(uint64_t* b, uint32_t ph, volat
         "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
         " selp.u32 %0,1,0,p;\n}\n" : "=r"(ok) : "r"(tc::saddr(b)), "r"(ph) : "memory");
     if (ok) return true;
-    if (*fail) return false;
+    if (fail && *fail) return false;
     if (n > (1u << 22)) {
-      *fail = 1;
+      if (fail) *fail = 1;
       atomicExch(err, code);
       return false;
     }
   }
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+// (relaxed: what it orders is mbarrier initialisation, which has its own fence)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
