@@ -48,15 +48,16 @@ constexpr int kSkThreads = 64 + kEpi * 32;
 constexpr int kErrSk = 0x6b40;
 
 // ------------------------------------------------------------------------------------------------------ expansion
-// 16 elements (bf16 pairs) of a block with exponent e -> word t of each term: 8 bytes of codes.  X' = X + sum_t 4 * 8^t has
-// the digits d_t + 4 as its octal digits; a byte permutation looks up the codes of 4 digits at a time, even elements in
-// the low and odd ones in the high nibble.
+// 8 elements (bf16 pairs) of a block with exponent e -> per term a word of 8 codes.  X' = X + sum_t 4 * 8^t has the digits
+// d_t + 4 as its octal digits; a byte permutation looks up the codes of 4 digits at a time, even elements in the low and
+// odd ones in the high nibble.
 template <typename F>
-__device__ __forceinline__ void expand16(const uint32_t (&w)[8], int e, F&& emit) {
+__device__ __forceinline__ void expand8(const uint4& w4, int e, F&& emit) {
+  const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
   const float s = pow2i(21 - e);
-  uint32_t x[16];
+  uint32_t x[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     // 1.5 * 2^23 + X: X in the low bits of the float
     constexpr uint32_t kShift = 044444444u - 0x4b400000u;
     x[2 * i] = __float_as_uint(fmaf(__uint_as_float(w[i] << 16), s, 12582912.f)) + kShift;
@@ -65,38 +66,35 @@ __device__ __forceinline__ void expand16(const uint32_t (&w)[8], int e, F&& emit
 #pragma unroll
   for (int t = 0; t < kTerms; ++t) {
     const int sh = 3 * (kTerms - 1 - t);
-    uint32_t code[2];
+    uint32_t lo = 0, hi = 0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t lo = 0, hi = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t a = x[8 * h + 2 * i], b = x[8 * h + 2 * i + 1];
-        lo |= (sh >= 4 * i ? a >> (sh - 4 * i) : a << (4 * i - sh)) & (7u << (4 * i));
-        hi |= (sh >= 4 * i ? b >> (sh - 4 * i) : b << (4 * i - sh)) & (7u << (4 * i));
-      }
-      // codes of the digits -4 -3 -2 -1 0 1 2 3: 14 13 12 10 0 2 4 5
-      code[h] = __byte_perm(0x0a0c0d0eu, 0x05040200u, lo) | __byte_perm(0xa0c0d0e0u, 0x50402000u, hi);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = x[2 * i], b = x[2 * i + 1];
+      lo |= (sh >= 4 * i ? a >> (sh - 4 * i) : a << (4 * i - sh)) & (7u << (4 * i));
+      hi |= (sh >= 4 * i ? b >> (sh - 4 * i) : b << (4 * i - sh)) & (7u << (4 * i));
     }
-    emit(t, make_uint2(code[0], code[1]));
+    // codes of the digits -4 -3 -2 -1 0 1 2 3: 14 13 12 10 0 2 4 5
+    emit(t, __byte_perm(0x0a0c0d0eu, 0x05040200u, lo) | __byte_perm(0xa0c0d0e0u, 0x50402000u, hi));
   }
 }
 
-__device__ __forceinline__ uint32_t amax_bits16(const uint32_t (&w)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
-  return m;
+__device__ __forceinline__ uint32_t amax_bits8(const uint4& w) {
+  const uint32_t a = max_u16x2(max_u16x2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
+                               max_u16x2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+  return max(a << 16, a & 0xffff0000u);
 }
-__device__ __forceinline__ void load16(const uint16_t* x, bool vec, uint32_t (&w)[8]) {
-  if (vec) {
-    const uint4 a = *reinterpret_cast<const uint4*>(x), c = *reinterpret_cast<const uint4*>(x + 8);
-    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-    w[4] = c.x; w[5] = c.y; w[6] = c.z; w[7] = c.w;
-  } else {
+// largest over the threads of a block: two (16 elements) or four (32)
+template <bool NV>
+__device__ __forceinline__ uint32_t block_amax(uint32_t am) {
+  am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
+  return NV ? am : max(am, __shfl_xor_sync(0xffffffffu, am, 2));
+}
+__device__ __forceinline__ uint4 load8(const uint16_t* x, bool vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(x);
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = (uint32_t)x[2 * i] | ((uint32_t)x[2 * i + 1] << 16);
-  }
+  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)x[2 * i] | ((uint32_t)x[2 * i + 1] << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ int exponent(uint32_t bits) { return (int)(bits >> 23) - 127; }
 // nvfp4: exponent of the row, low enough rows share one (2^(21-e) stays in range)
@@ -105,7 +103,7 @@ __device__ __forceinline__ float row_factor(uint32_t amax) {
   return amax >= kInfBits ? __uint_as_float(0x7fc00000u) : pow2i(max(row_exponent(amax) - 8, -126));
 }
 
-// block of 16 -> exponent and scale byte(s).  nvfp4: one byte for all terms (the term's 2^-3t is put back later); mxfp4:
+// largest magnitude of a block -> exponent and scale byte(s).  nvfp4: one byte for all terms (the term's 2^-3t is put back later); mxfp4:
 // byte of term 0, term t is 3t lower
 template <bool NV>
 __device__ __forceinline__ int block_exponent(uint32_t amax, int row_e, uint32_t& byte) {
@@ -135,7 +133,7 @@ __device__ __forceinline__ uint32_t term_scales(uint32_t s4, int t) {
 // scale bytes of four neighbouring columns in one word (valid in the first of their lanes)
 template <bool NV>
 __device__ __forceinline__ uint32_t gather_scales(uint32_t sc) {
-  constexpr int kStep = NV ? 1 : 2;
+  constexpr int kStep = NV ? 2 : 4;
   uint32_t s4 = sc;
   s4 |= __shfl_down_sync(0xffffffffu, sc, kStep) << 8;
   s4 |= __shfl_down_sync(0xffffffffu, sc, 2 * kStep) << 16;
@@ -143,48 +141,42 @@ __device__ __forceinline__ uint32_t gather_scales(uint32_t sc) {
   return s4;
 }
 
-// CTA: 128 blocks of 16 of one row (a thread each); nvfp4 reads the whole row for its maximum first
+// CTA: 256 times 8 elements of one row; nvfp4 reads the whole row for its maximum first
 template <bool NV>
-__global__ void __launch_bounds__(128) fp4_expand_kernel(Fp4ExpandArgs p) {
-  __shared__ uint32_t red[4];
-  const int m = blockIdx.y, b = blockIdx.x * 128 + threadIdx.x;
+__global__ void __launch_bounds__(256) fp4_expand_kernel(Fp4ExpandArgs p) {
+  __shared__ uint32_t red[8];
+  const int m = blockIdx.y, b = blockIdx.x * 256 + threadIdx.x;
   const int KT = tiles_k(p.K);
-  const int nb = KT * 16, nk = p.K / 16;
+  const int nk = p.K / 8;
   const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + (int64_t)m * p.ldx;
   pdl_trigger();
   pdl_wait();
-  uint32_t w[8];
+  const uint4 w = b < nk ? load8(x + (int64_t)b * 8, p.vec) : make_uint4(0, 0, 0, 0);
   int row_e = 0;
   if constexpr (NV) {
     uint32_t am = 0;
-    for (int blk = threadIdx.x; blk < nk; blk += 128) {
-      load16(x + (int64_t)blk * 16, p.vec, w);
-      am = max(am, amax_bits16(w));
-    }
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nk; i += 256) am = max(am, amax_bits8(load8(x + (int64_t)i * 8, p.vec)));
     am = __reduce_max_sync(0xffffffffu, am);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = am;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) am = max(am, red[i]);
+    for (int i = 0; i < 8; ++i) am = max(am, red[i]);
     row_e = row_exponent(am);
     if (b == 0) p.factor[m] = row_factor(am);
   } else if (b == 0) {
     p.factor[m] = 1.f;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = 0u;
-  if (b < nk) load16(x + (int64_t)b * 16, p.vec, w);
-  uint32_t am = amax_bits16(w), sc;
-  if (!NV) am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
-  const int e = block_exponent<NV>(am, row_e, sc);
+  uint32_t sc;
+  const int e = block_exponent<NV>(block_amax<NV>(amax_bits8(w)), row_e, sc);
   const uint32_t s4 = gather_scales<NV>(b < nk ? sc : 0u);
-  const int kt = b >> 4, kb = b & 15;
-  if (b < nb)
-    expand16(w, e, [&](int t, uint2 code) {
+  const int kt = b >> 5, kb = b & 31;
+  if (kt < KT)
+    expand8(w, e, [&](int t, uint32_t code) {
       const int row = m * kTerms + t, rr = row % kTileRows;
       const int64_t tile = (int64_t)(row / kTileRows) * KT + kt;
-      *reinterpret_cast<uint2*>(p.codes + tile * kTileBytes + chunk_off(rr, kb >> 1) + (kb & 1) * 8) = code;
-      constexpr int kStep = NV ? 1 : 2;
+      *reinterpret_cast<uint32_t*>(p.codes + tile * kTileBytes + chunk_off(rr, kb >> 2) + (kb & 3) * 4) = code;
+      constexpr int kStep = NV ? 2 : 4;
       if ((kb & (4 * kStep - 1)) == 0)
         *reinterpret_cast<uint32_t*>(p.scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, kb / kStep)) =
             term_scales<NV>(s4, t);
@@ -334,13 +326,16 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
     if (elect_one()) {
       const int ksteps = (p.K + 63) / 64;
       uint32_t it = 0, blk = 0;
-      bool ok = !INLINE || sk_wait(&xready, 0, stop);
+      bool ok = true;
       for (int nb = cid; nb < pl.blocks && ok; nb += pl.clusters, ++blk) {
         if (blk > 0 && !sk_wait(&tempty, (blk - 1) & 1, stop)) break;
         tc::fence_after();
         for (int t = t_lo; t < t_hi; ++t, ++it) {
           const int s = it % pl.stages;
-          if (!sk_wait(&full[s], (it / pl.stages) & 1, stop)) { ok = false; break; }
+          if (!sk_wait(&full[s], (it / pl.stages) & 1, stop) || (INLINE && it == 0 && !sk_wait(&xready, 0, stop))) {
+            ok = false;
+            break;
+          }
           tc::fence_after();
           const uint32_t a = tc::saddr(ring + s * pl.stage_bytes);
           const uint32_t xc = INLINE ? tc::saddr(xs + (t - t_lo) * xtile) : a + off_x;
@@ -381,35 +376,36 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
     const int buf_floats = CL * 2 * j_per * Mp;
     const bool swi = p.mode == GEMV_SWIGLU;
     const bool direct = CL == 1 && !swi;              // rows finished where they are read
+    // this thread's first share of the finishing: four tokens of one row (of a pair of rows)
+    const int f_q = et / rows, f_row = et - f_q * rows, f_half = swi ? 0 : f_q & 1;
     pdl_wait();
     if constexpr (INLINE) {
-      // a thread per block of 16 of the slice (the plan sees to it that there are no more than threads)
-      const int nblk = (t_hi - t_lo) * 16, nk = p.K / 16 - t_lo * 16;       // blocks in the slice; those that exist
+      // a thread per 8 elements of the slice (the plan sees to it that there are no more than threads)
+      const int nblk = (t_hi - t_lo) * 32, nk = p.K / 8 - t_lo * 32;        // eights in the slice; those that exist
       const bool in = et < p.M * nblk;
       const int m = in ? et / nblk : 0, b = et - m * nblk;
-      uint32_t w[8] = {};
+      uint4 w = make_uint4(0, 0, 0, 0);
       if (in && b < nk)
-        load16(reinterpret_cast<const uint16_t*>(p.x) + (int64_t)m * p.ldx + (int64_t)t_lo * kTileK + b * 16, p.xvec, w);
-      uint32_t am = amax_bits16(w), sc;
+        w = load8(reinterpret_cast<const uint16_t*>(p.x) + (int64_t)m * p.ldx + (int64_t)t_lo * kTileK + b * 8, p.xvec);
+      const uint32_t am = amax_bits8(w);
       if constexpr (NV) {
-        // the 16 lanes of a half warp belong to one row
-        const uint32_t hm = __reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, am);
-        if (in && (lane & 15) == 0) atomicMax(&xmax[m], hm);
+        // a warp's lanes belong to one row
+        const uint32_t wm = __reduce_max_sync(0xffffffffu, am);
+        if (in && lane == 0) atomicMax(&xmax[m], wm);
         sk_sync();
         if (et < p.M) xfac[et] = row_factor(xmax[et]);
-      } else {
-        am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
       }
-      const int e = block_exponent<NV>(am, NV ? row_exponent(xmax[m]) : 0, sc);
+      uint32_t sc;
+      const int e = block_exponent<NV>(block_amax<NV>(am), NV ? row_exponent(xmax[m]) : 0, sc);
       const uint32_t s4 = gather_scales<NV>(b < nk ? sc : 0u);
       if (in) {
-        const int kb = b & 15;
-        uint8_t* xc = xs + (b >> 4) * xtile;
-        uint8_t* xsc = xs + pl.per * xtile + (b >> 4) * kSB;
-        expand16(w, e, [&](int t, uint2 code) {
+        const int kb = b & 31;
+        uint8_t* xc = xs + (b >> 5) * xtile;
+        uint8_t* xsc = xs + pl.per * xtile + (b >> 5) * kSB;
+        expand8(w, e, [&](int t, uint32_t code) {
           const int row = m * kTerms + t;
-          *reinterpret_cast<uint2*>(xc + chunk_off(row, kb >> 1) + (kb & 1) * 8) = code;
-          constexpr int kStep = NV ? 1 : 2;
+          *reinterpret_cast<uint32_t*>(xc + chunk_off(row, kb >> 2) + (kb & 3) * 4) = code;
+          constexpr int kStep = NV ? 2 : 4;
           if ((kb & (4 * kStep - 1)) == 0)
             *reinterpret_cast<uint32_t*>(xsc + scale_off(row, kb / kStep)) = term_scales<NV>(s4, t);
         });
@@ -427,9 +423,11 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
     for (int nb = cid; nb < pl.blocks; nb += pl.clusters, ++blk) {
       const uint32_t rbar = tc::saddr(&recv_bar[blk & 1]);
       if (CL > 1 && et == 0) bulk_expect(&recv_bar[blk & 1], (uint32_t)((CL - 1) * 2 * rows * Mp * 4));
-      // scale of this thread's row: loaded under the main loop
-      float rs = 1.f;
-      if (NV && direct && nb * 128 + r < p.N) rs = __ldcg(p.row_scale + nb * 128 + r);
+      // scales of the rows that this thread finishes (first): loaded under the main loop
+      float rs = 1.f, ru = 1.f;
+      const int n_own = nb * 128 + (direct ? r : j_lo + f_row + f_half * 64);
+      if (NV && n_own < p.N) rs = __ldcg(p.row_scale + n_own);
+      if (NV && swi && n_own + 64 < p.N) ru = __ldcg(p.row_scale + n_own + 64);
       if (!dead) {
         int ok = 0;
         if (lane == 0) ok = sk_wait(&tfull, blk & 1, stop) ? 1 : 0;
@@ -474,7 +472,8 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       // ---- finish rows j_lo.. and + 64, four tokens at a time: consecutive threads on consecutive rows
       const int units = rows * (Mp / 4) * (swi ? 1 : 2);
       for (int e = et; e < units; e += kEpi * 32) {
-        const int q = e / rows, row = e - q * rows;
+        const bool own = e == et;
+        const int q = own ? f_q : e / rows, row = own ? f_row : e - q * rows;
         const int tok = (swi ? q : q >> 1) * 4, hf = swi ? 0 : q & 1;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
         for (int c = 0; c < CL; ++c) {
@@ -492,7 +491,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
         if (swi) {
           const int col = nb * 64 + j_lo + row;
           if (col >= p.width) continue;
-          const float sg = NV ? __ldcg(p.row_scale + n) : 1.f, su = NV ? __ldcg(p.row_scale + n + 64) : 1.f;
+          const float sg = !NV || own ? rs : __ldcg(p.row_scale + n), su = !NV || own ? ru : __ldcg(p.row_scale + n + 64);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (tok + i >= p.M) break;
@@ -504,7 +503,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
           }
         } else {
           if (n >= p.N) continue;
-          const float sc = NV ? __ldcg(p.row_scale + n) : 1.f;
+          const float sc = !NV || own ? rs : __ldcg(p.row_scale + n);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (tok + i < p.M) store1(p, tok + i, n, vs[i] * sc);
@@ -585,7 +584,7 @@ static cudaError_t sk_plan(int M, int64_t N, int K, int dev, SkPlan& b, double& 
   for (int cl = 1; cl <= 8 && cl <= b.KT; ++cl) {
     const int per = (b.KT + cl - 1) / cl;
     if ((b.KT + per - 1) / per != cl) continue;       // a CTA of the cluster would have no tile
-    if (INLINE && M * per * 16 > kEpi * 32) continue;
+    if (INLINE && M * per * 32 > kEpi * 32) continue;  // a thread per 8 elements
     int active = 0;
     const cudaError_t e = sk_active<WIDE>(dev, cl, &active);
     if (e != cudaSuccess) return e;
@@ -671,9 +670,9 @@ bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv) {
 
 cudaError_t g53_fp4_expand(const Fp4ExpandArgs& p, cudaStream_t st) {
   if (p.M < 1 || p.M > 32 || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
-  const dim3 grid((fp4::tiles_k(p.K) * 16 + 127) / 128, p.M);
-  return p.nv ? g53_launch_pdl(fp4::fp4_expand_kernel<true>, grid, dim3(128), 0, st, 1, p)
-              : g53_launch_pdl(fp4::fp4_expand_kernel<false>, grid, dim3(128), 0, st, 1, p);
+  const dim3 grid((fp4::tiles_k(p.K) * 32 + 255) / 256, p.M);
+  return p.nv ? g53_launch_pdl(fp4::fp4_expand_kernel<true>, grid, dim3(256), 0, st, 1, p)
+              : g53_launch_pdl(fp4::fp4_expand_kernel<false>, grid, dim3(256), 0, st, 1, p);
 }
 
 cudaError_t g53_fp4_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
