@@ -19,8 +19,10 @@ using OptT = c10::optional<Tensor>;
 
 constexpr int64_t kTileRows = 128, kTileK = 256, kTileBytes = 16384;
 constexpr int64_t kFourRows = 16;      // rows above which act4 quantises the activations
-constexpr int64_t kSkinnyRows = 32;    // rows of one small-M launch
-constexpr int64_t kGemmRows = 64;      // rows from which exact activations go through the bf16 tcgen05 GEMM
+constexpr int64_t kGemmRows = 256;     // rows above which exact activations go through the bf16 tcgen05 GEMM (4096 x 4096: 200
+                                       // rows 28.5 us, 34.5 there; 300 rows 37.6, 34.6)
+constexpr int64_t kFour = 128;         // rows up to which 4-bit activations go through the small-M kernel (24576 x 4096: 100 rows
+                                       // 28.8 us, 36.3 on the GEMM; 200 rows 42.6, 35.5)
 
 void ok(cudaError_t e, const char* what) {
   TORCH_CHECK(e == cudaSuccess, "glm53 kernel ", what, " failed: ", cudaGetErrorString(e));
@@ -167,49 +169,64 @@ void check_xy(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int
               op, ": y must be [", num(x.size(0)), ", ", num(n), "], rows contiguous and apart");
 }
 
-// all rows of x through the small-M kernel, kSkinnyRows at a time
-void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t width, int64_t mode, double limit) {
-  const int64_t K = w.k, sb = scale_bytes(w.nv);
-  for (int64_t m0 = 0; m0 < x.size(0); m0 += kSkinnyRows) {
-    const int64_t m = std::min(kSkinnyRows, x.size(0) - m0);
-    const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()) + m0 * x.stride(0);
-    const int vec = aligned16(rows) && x.stride(0) % 8 == 0;
-    Fp4SkinnyArgs a{};
-    Tensor buf;
-    if (g53_fp4_expand_inline((int)m, n, (int)K, w.nv)) {
-      a.x = rows;
-      a.ldx = x.stride(0);
-      a.xvec = vec;
-    } else {
-      const int64_t tiles = n_tiles(m * g53_fp4_terms(), K);
-      buf = at::empty({tiles * (kTileBytes + sb) + m * 4}, x.options().dtype(at::kByte));
-      uint8_t* b = buf.data_ptr<uint8_t>();
-      Fp4ExpandArgs e{};
-      e.x = rows;
-      e.ldx = x.stride(0);
-      e.M = (int)m;
-      e.K = (int)K;
-      e.nv = w.nv;
-      e.vec = vec;
-      a.x_codes = e.codes = b;
-      a.x_scales = e.scales = b + tiles * kTileBytes;
-      a.x_factor = e.factor = reinterpret_cast<float*>(b + tiles * (kTileBytes + sb));
-      ok(g53_fp4_expand(e, stream()), "fp4_expand");
-    }
-    a.codes = w.codes;
-    a.scales = w.scales;
-    a.row_scale = w.row_scale;
-    a.nv = w.nv;
-    a.y = reinterpret_cast<uint8_t*>(y.data_ptr()) + m0 * y.stride(0) * y.element_size();
-    a.ldy = y.stride(0);
-    a.M = (int)m;
-    a.N = (int)n;
-    a.K = (int)K;
-    a.width = (int)width;
-    a.mode = (int)mode;
-    a.limit = (float)limit;
-    ok(g53_fp4_skinny(a, stream()), "fp4_skinny");
+// small-M product: the arguments that do not depend on the form of x
+Fp4SkinnyArgs skinny_args(int64_t M, const Matrix4& w, const Tensor& y, int64_t width, int64_t mode, double limit) {
+  Fp4SkinnyArgs a{};
+  a.codes = w.codes;
+  a.scales = w.scales;
+  a.row_scale = w.row_scale;
+  a.nv = w.nv;
+  a.y = y.data_ptr();
+  a.ldy = y.stride(0);
+  a.M = (int)M;
+  a.N = (int)w.rows;
+  a.K = (int)w.k;
+  a.width = (int)width;
+  a.mode = (int)mode;
+  a.limit = (float)limit;
+  return a;
+}
+
+// exact activations, few rows: expanded into 4-bit terms, by the product itself or in a launch of their own
+void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t width, int64_t mode, double limit) {
+  Fp4SkinnyArgs a = skinny_args(x.size(0), w, y, width, mode, limit);
+  const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
+  const int vec = aligned16(rows) && x.stride(0) % 8 == 0;
+  Tensor buf;
+  if (g53_fp4_expand_inline(a.M, a.N, a.K, a.nv)) {
+    a.x = rows;
+    a.ldx = x.stride(0);
+    a.xvec = vec;
+  } else {
+    // whole groups of 256 image rows: the product fetches them
+    const int64_t tiles = n_tiles((x.size(0) * g53_fp4_terms() + 255) / 256 * 256, w.k);
+    buf = at::empty({tiles * (kTileBytes + scale_bytes(w.nv)) + a.M * 4}, x.options().dtype(at::kByte));
+    uint8_t* b = buf.data_ptr<uint8_t>();
+    Fp4ExpandArgs e{};
+    e.x = rows;
+    e.ldx = x.stride(0);
+    e.M = a.M;
+    e.K = a.K;
+    e.nv = a.nv;
+    e.vec = vec;
+    a.x_codes = e.codes = b;
+    a.x_scales = e.scales = b + tiles * kTileBytes;
+    a.x_factor = e.factor = reinterpret_cast<float*>(b + tiles * (kTileBytes + scale_bytes(w.nv)));
+    a.terms = g53_fp4_terms();
+    ok(g53_fp4_expand(e, stream()), "fp4_expand");
   }
+  ok(g53_fp4_skinny(a, stream()), "fp4_skinny");
+}
+
+// 4-bit activations, few rows; `factor`: the row scale of all rows, where x has none of its own
+void skinny4(const Matrix4& x, float factor, const Matrix4& w, const Tensor& y, int64_t mode) {
+  Fp4SkinnyArgs a = skinny_args(x.rows, w, y, 0, mode, 0.0);
+  a.x_codes = x.codes;
+  a.x_scales = x.scales;
+  a.x_factor = factor == 1.f ? x.row_scale : nullptr;
+  a.x_const = factor;
+  a.terms = 1;
+  ok(g53_fp4_skinny(a, stream()), "fp4_skinny");
 }
 
 // exact activations, many rows: the weights widened to bf16 (every 4-bit value times its scales is a bf16 value), then
@@ -230,6 +247,9 @@ void gemm_exact(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, i
   p.K = (int)w.k;
   p.mode = (int)mode;
   p.limit = (float)limit;
+  // 128-column tiles where they still are one wave (500 x 4096 x 12288: 93 us, 107 with 256; where they are two, 300 rows
+  // of 24576 x 4096 stay at 121 and 800 of 4096 x 4096 would take 57 instead of 38)
+  if ((x.size(0) + 127) / 128 * ((n + 127) / 128) <= at::cuda::getCurrentDeviceProperties()->multiProcessorCount) p.bn = 128;
   ok(g53_fp4_gemm_error_word(&p.err), "fp4 error word");
   ok(g53_gemm_sm100(p, stream()), "gemm_sm100");
 }
@@ -258,14 +278,18 @@ void linear(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t mode, bo
   const c10::cuda::CUDAGuard guard(x.device());
   if (M > kFourRows && act4) {
     const Matrix4 a = quantize(x, w.nv);
+    if (M <= kFour) {
+      skinny4(a, 1.f, w, y, mode);
+      return;
+    }
     Fp4GemmArgs p = gemm_args(a, w, mode);
     p.y = y.data_ptr();
     p.ldy = y.stride(0);
     ok(g53_fp4_gemm(p, stream()), "fp4_gemm");
-  } else if (M >= kGemmRows) {
+  } else if (M > kGemmRows) {
     gemm_exact(x, w, y, w.rows, 0, mode, 0.0);
   } else {
-    skinny(x, w, y, w.rows, 0, mode, 0.0);
+    skinny(x, w, y, 0, mode, 0.0);
   }
 }
 
@@ -301,22 +325,27 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
     p.out_scales = h.scales;
     p.h_exp = gu.nv ? row_exp(l2) : 0;
     ok(g53_fp4_gemm(p, stream()), "fp4_gemm");
+    const float factor = gu.nv ? std::ldexp(1.f, p.h_exp) : 1.f;
+    if (M <= kFour) {
+      skinny4(h, factor, down, y, mode);
+      return;
+    }
     Fp4GemmArgs d = gemm_args(h, down, mode);
     d.a_row = nullptr;
-    d.a_const = gu.nv ? std::ldexp(1.f, p.h_exp) : 1.f;
+    d.a_const = factor;
     d.y = y.data_ptr();
     d.ldy = y.stride(0);
     ok(g53_fp4_gemm(d, stream()), "fp4_gemm");
     return;
   }
   const Tensor h = at::empty({M, W}, x.options());
-  if (M >= kGemmRows) {
+  if (M > kGemmRows) {
     gemm_exact(x, gu, h, 2 * W, W, GEMV_SWIGLU_F32, limit);
     gemm_exact(h, down, y, down.rows, 0, mode, 0.0);
     return;
   }
-  skinny(x, gu, h, gu.rows, W, GEMV_SWIGLU, limit);
-  skinny(h, down, y, down.rows, 0, mode, 0.0);
+  skinny(x, gu, h, W, GEMV_SWIGLU, limit);
+  skinny(h, down, y, 0, mode, 0.0);
 }
 
 int64_t error(int64_t device) {

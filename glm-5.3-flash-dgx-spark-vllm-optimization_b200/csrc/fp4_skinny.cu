@@ -185,10 +185,10 @@ __global__ void __launch_bounds__(256) fp4_expand_kernel(Fp4ExpandArgs p) {
 
 // -------------------------------------------------------------------------------------------------------- product
 // per: K tiles of a slice; stages: ring depth; clusters: persistent clusters; ncol: mma N; xbytes: resident expansion
+// units: row blocks x groups of (at most `group`) rows of x, each served by one pass over a weight tile
 struct SkPlan {
-  int blocks, KT, per, stages, clusters, CL, ncol, stage_bytes, xbytes;
+  int units, groups, group, KT, per, stages, clusters, CL, ncol, stage_bytes, xbytes;
 };
-
 __device__ __forceinline__ bool sk_wait(uint64_t* b, uint32_t ph, volatile int* stop, bool drain = false) {
   uint32_t n = 0;
   while (!tc::bar_try(b, ph)) {
@@ -228,18 +228,19 @@ __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
   return r;
 }
 
-// WIDE: mma N up to 256 (17..32 rows), one CTA per SM; otherwise N <= 128 and two CTAs per SM
-template <bool NV, bool WIDE, bool INLINE>
+// T: terms per row of x: 8 (expanded), or 1 (4-bit rows as they are).  WIDE: mma N up to 256, one CTA per SM; otherwise N
+// <= 128 and two CTAs per SM
+template <bool NV, int T, bool WIDE, bool INLINE>
 __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp4SkinnyArgs p, SkPlan pl) {
   constexpr int kSB = Fmt<NV>::kScaleBytes;
   constexpr int kAtoms = kSB / 512;
-  constexpr int kXB = WIDE ? 2 : 1;                   // 128-row blocks of the expansion
+  constexpr int kXB = WIDE && T > 1 ? 2 : 1;          // 128-row blocks of X per group
   constexpr uint32_t kCols = WIDE ? 512 : 256;        // TMEM columns: sums, scales of W, scales of X
   constexpr uint32_t kSfW = WIDE ? 256 : 128, kSfX = kSfW + 16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[8], empty[8], recv_bar[2], tfull, tempty, xready, drain;
   __shared__ uint32_t tmem_s, xmax[32];
-  __shared__ float xfac[32 + 4];                      // read four at a time
+  __shared__ float xfac[32];
   __shared__ int stop_s;
   volatile int* stop = &stop_s;
   uint8_t* xs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
   const int j_per = (64 + CL - 1) / CL;
   const int j_lo = min(64, rank * j_per), rows = min(64, j_lo + j_per) - j_lo;
   const int xrows = pl.ncol;                          // rows of the expansion
-  const int xb0 = min(xrows, 128) * 128, xb1 = WIDE ? max(0, xrows - 128) * 128 : 0;
+  const int xb0 = min(xrows, 128) * 128, xb1 = kXB == 2 ? max(0, xrows - 128) * 128 : 0;
   const int xtile = xrows * 128;                      // code bytes of the expansion per K tile
   // a stage: codes of W, (codes of X,) scales of W, (scales of X)
   const int off_x = kTileBytes, off_sw = off_x + (INLINE ? 0 : xtile), off_sx = off_sw + kSB;
@@ -286,30 +287,34 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
   if (warp == 0) {
     if (elect_one()) {
       const uint64_t pol = l2_evict_first_policy();
-      for (int t = t_lo; t < t_hi && t < t_lo + 8 && cid < pl.blocks; ++t) {
-        const int64_t tile = (int64_t)cid * pl.KT + t;
+      for (int t = t_lo; t < t_hi && t < t_lo + 8; ++t) {
+        const int64_t tile = (int64_t)(cid / pl.groups) * pl.KT + t;
         sk_prefetch(p.codes + tile * kTileBytes, kTileBytes);
         sk_prefetch(p.scales + tile * kSB, kSB);
       }
       pdl_wait();
       uint32_t it = 0;
       bool ok = true;
-      for (int nb = cid; nb < pl.blocks && ok; nb += pl.clusters) {
+      for (int u = cid; u < pl.units && ok; u += pl.clusters) {
+        const int nb = u / pl.groups;
+        const int xrow = (u - nb * pl.groups) * pl.group * T;                // first image row of X: a multiple of 64
+        const int64_t xblk = (int64_t)(xrow / kTileRows) * pl.KT;
+        const int xoff = (xrow & 64) * 128;
         for (int t = t_lo; t < t_hi; ++t, ++it) {
           const int s = it % pl.stages;
           const uint32_t round = it / pl.stages;
           if (round > 0 && !sk_wait(&empty[s], (round - 1) & 1, stop)) { ok = false; break; }
           uint8_t* dst = ring + s * pl.stage_bytes;
-          bulk_expect(&full[s], (uint32_t)(kTileBytes + kSB + (INLINE ? 0 : xb0 + kSB + (WIDE && xb1 ? xb1 + kSB : 0))));
+          bulk_expect(&full[s], (uint32_t)(kTileBytes + kSB + (INLINE ? 0 : xb0 + kSB + (xb1 ? xb1 + kSB : 0))));
           const int64_t tw = (int64_t)nb * pl.KT + t;
           bulk_load_hint(dst, p.codes + tw * kTileBytes, kTileBytes, &full[s], pol);
           bulk_load_hint(dst + off_sw, p.scales + tw * kSB, kSB, &full[s], pol);
           if constexpr (!INLINE) {
-            bulk_load(dst + off_x, p.x_codes + (int64_t)t * kTileBytes, xb0, &full[s]);
-            bulk_load(dst + off_sx, p.x_scales + (int64_t)t * kSB, kSB, &full[s]);
-            if (WIDE && xb1) {
-              bulk_load(dst + off_x + kTileBytes, p.x_codes + (int64_t)(pl.KT + t) * kTileBytes, xb1, &full[s]);
-              bulk_load(dst + off_sx + kSB, p.x_scales + (int64_t)(pl.KT + t) * kSB, kSB, &full[s]);
+            bulk_load(dst + off_x, p.x_codes + (xblk + t) * kTileBytes + xoff, xb0, &full[s]);
+            bulk_load(dst + off_sx, p.x_scales + (xblk + t) * kSB, kSB, &full[s]);
+            if (kXB == 2 && xb1) {
+              bulk_load(dst + off_x + kTileBytes, p.x_codes + (xblk + pl.KT + t) * kTileBytes, xb1, &full[s]);
+              bulk_load(dst + off_sx + kSB, p.x_scales + (xblk + pl.KT + t) * kSB, kSB, &full[s]);
             }
           }
         }
@@ -327,7 +332,9 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       const int ksteps = (p.K + 63) / 64;
       uint32_t it = 0, blk = 0;
       bool ok = true;
-      for (int nb = cid; nb < pl.blocks && ok; nb += pl.clusters, ++blk) {
+      for (int u = cid; u < pl.units && ok; u += pl.clusters, ++blk) {
+        // rows 64.. of a 128-row block of X: the second half of its scale columns
+        const uint32_t sfx = tmem + kSfX + (((u % pl.groups) * pl.group * T) & 64 ? 2 : 0);
         if (blk > 0 && !sk_wait(&tempty, (blk - 1) & 1, stop)) break;
         tc::fence_after();
         for (int t = t_lo; t < t_hi; ++t, ++it) {
@@ -354,7 +361,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
             const int at = NV ? k : k >> 1;
             const uint32_t sf = NV ? 0u : (uint32_t)(k & 1) * 2;
             mma4<NV>(tmem, tc::desc_sw128(a + k * 32), tc::desc_sw128(xc + k * 32), idesc4(128, pl.ncol, !NV, sf),
-                     tmem + kSfW + at * 4, tmem + kSfX + at * (4 * kXB), (t > t_lo || k > 0) ? 1u : 0u);
+                     tmem + kSfW + at * 4, sfx + at * (4 * kXB), (t > t_lo || k > 0) ? 1u : 0u);
           }
           tc::commit(&empty[s]);
         }
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
     const int r = quad * 32 + lane;                   // row of the block
     const int j = r & 63, half = r >> 6;
     const int owner = j / j_per, jl = j - owner * j_per;
-    const int Mp = (p.M + 3) & ~3;
+    const int Mp = (min(p.M, pl.group) + 3) & ~3;      // rows of x in a group, rounded up to fours
     const int buf_floats = CL * 2 * j_per * Mp;
     const bool swi = p.mode == GEMV_SWIGLU;
     const bool direct = CL == 1 && !swi;              // rows finished where they are read
@@ -413,21 +420,31 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       tc::fence_async_smem();
       __syncwarp();
       if (lane == 0) tc::bar_arrive(&xready);
-    } else {
-      if (NV && et < p.M) xfac[et] = p.x_factor[et];
     }
     if (CL > 1) cluster_wait();                       // every CTA of the cluster has its barriers
     sk_sync();
     uint32_t blk = 0;
     bool dead = false;
-    for (int nb = cid; nb < pl.blocks; nb += pl.clusters, ++blk) {
+    for (int u = cid; u < pl.units; u += pl.clusters, ++blk) {
+      const int nb = u / pl.groups, x0 = (u - nb * pl.groups) * pl.group;  // first row of x
+      const int M = min(p.M - x0, pl.group);
       const uint32_t rbar = tc::saddr(&recv_bar[blk & 1]);
-      if (CL > 1 && et == 0) bulk_expect(&recv_bar[blk & 1], (uint32_t)((CL - 1) * 2 * rows * Mp * 4));
+      if (CL > 1 && et == 0) bulk_expect(&recv_bar[blk & 1], (uint32_t)((CL - 1) * 2 * rows * ((M + 3) & ~3) * 4));
       // scales of the rows that this thread finishes (first): loaded under the main loop
       float rs = 1.f, ru = 1.f;
       const int n_own = nb * 128 + (direct ? r : j_lo + f_row + f_half * 64);
       if (NV && n_own < p.N) rs = __ldcg(p.row_scale + n_own);
       if (NV && swi && n_own + 64 < p.N) ru = __ldcg(p.row_scale + n_own + 64);
+      // factors of the rows of x: lane l those of l, l + 32, ..
+      constexpr int kXf = T == 1 ? 4 : 1;
+      float xf[kXf];
+#pragma unroll
+      for (int i = 0; i < kXf; ++i) {
+        xf[i] = 1.f;
+        if (NV && INLINE) xf[i] = xfac[lane];
+        if (NV && !INLINE && lane + 32 * i < M)
+          xf[i] = p.x_factor ? __ldcg(p.x_factor + x0 + lane + 32 * i) : p.x_const;
+      }
       if (!dead) {
         int ok = 0;
         if (lane == 0) ok = sk_wait(&tfull, blk & 1, stop) ? 1 : 0;
@@ -438,26 +455,36 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       // this rank's sums of row r -> [rank][half][jl][token] of the owner
       float* dst = rb + ((rank * 2 + half) * j_per + jl) * Mp;
       const uint32_t rdst = CL > 1 ? map_to(tc::saddr(dst), owner) : 0, rdbar = CL > 1 ? map_to(rbar, owner) : 0;
-      for (int m0 = part * 4; m0 < p.M; m0 += kEpi) {
+      constexpr int kTok = 32 / T;                     // rows of x in 32 columns
+      for (int c0 = part * kTok; c0 < M; c0 += kTok * (kEpi / 4)) {
+        float f = xf[0];                               // of the 32 rows that hold these
+#pragma unroll
+        for (int i = 1; i < kXf; ++i) f = c0 >= 32 * i ? xf[i] : f;
         float v[32];
-        if (!dead) tc::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + m0 * kTerms, v);
-        float sum[4];
+        if (!dead) tc::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + c0 * T, v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sum[i] = 0.f;
+        for (int j4 = 0; j4 < kTok; j4 += 4) {
+          const int m0 = c0 + j4;
+          if (m0 >= M) break;
+          float sum[4];
 #pragma unroll
-          for (int t = kTerms - 1; t >= 0; --t)       // small terms first
-            sum[i] = NV ? fmaf(v[i * kTerms + t], 1.f / (float)(1 << (3 * t)), sum[i]) : sum[i] + v[i * kTerms + t];
-          if (NV) sum[i] *= xfac[m0 + i];             // rows past M: never used
-        }
-        if (direct) {
+          for (int i = 0; i < 4; ++i) {
+            sum[i] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (m0 + i < p.M && nb * 128 + r < p.N) store1(p, m0 + i, nb * 128 + r, sum[i] * rs);
-        } else if (owner == rank) {
-          *reinterpret_cast<float4*>(dst + m0) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-        } else {
-          send4(rdst + m0 * 4, rdbar, sum);
+            for (int t = T - 1; t >= 0; --t)           // small terms first
+              sum[i] = NV ? fmaf(v[(j4 + i) * T + t], 1.f / (float)(1 << (3 * t)), sum[i]) : sum[i] + v[(j4 + i) * T + t];
+            // rows past M: never used
+            if (NV) sum[i] *= __shfl_sync(0xffffffffu, f, (m0 + i) & 31);
+          }
+          if (direct) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (m0 + i < M && nb * 128 + r < p.N) store1(p, x0 + m0 + i, nb * 128 + r, sum[i] * rs);
+          } else if (owner == rank) {
+            *reinterpret_cast<float4*>(dst + m0) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+          } else {
+            send4(rdst + m0 * 4, rdbar, sum);
+          }
         }
       }
       tc::fence_before();
@@ -470,43 +497,43 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
         if (!ok) *stop = 1;                           // (waited for in a stopped CTA, too)
       }
       // ---- finish rows j_lo.. and + 64, four tokens at a time: consecutive threads on consecutive rows
-      const int units = rows * (Mp / 4) * (swi ? 1 : 2);
-      for (int e = et; e < units; e += kEpi * 32) {
+      const int shares = rows * ((M + 3) / 4) * (swi ? 1 : 2);
+      for (int e = et; e < shares; e += kEpi * 32) {
         const bool own = e == et;
         const int q = own ? f_q : e / rows, row = own ? f_row : e - q * rows;
         const int tok = (swi ? q : q >> 1) * 4, hf = swi ? 0 : q & 1;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), w = v;
         for (int c = 0; c < CL; ++c) {
           const float* src = rb + ((c * 2 + hf) * j_per + row) * Mp + tok;
           const float4 a = *reinterpret_cast<const float4*>(src);
           v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
           if (swi) {
             const float4 b = *reinterpret_cast<const float4*>(src + j_per * Mp);
-            u.x += b.x; u.y += b.y; u.z += b.z; u.w += b.w;
+            w.x += b.x; w.y += b.y; w.z += b.z; w.w += b.w;
           }
         }
         const int n = nb * 128 + j_lo + row + hf * 64;
         float vs[4] = {v.x, v.y, v.z, v.w};
-        const float us[4] = {u.x, u.y, u.z, u.w};
+        const float us[4] = {w.x, w.y, w.z, w.w};
         if (swi) {
           const int col = nb * 64 + j_lo + row;
           if (col >= p.width) continue;
           const float sg = !NV || own ? rs : __ldcg(p.row_scale + n), su = !NV || own ? ru : __ldcg(p.row_scale + n + 64);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (tok + i >= p.M) break;
-            float g = vs[i] * sg, w = us[i] * su;
+            if (tok + i >= M) break;
+            float g = vs[i] * sg, h = us[i] * su;
             // written so that a NaN stays one
             g = g > p.limit ? p.limit : g;
-            w = w > p.limit ? p.limit : w < -p.limit ? -p.limit : w;
-            reinterpret_cast<__nv_bfloat16*>(p.y)[(int64_t)(tok + i) * p.ldy + col] = f2bf(siluf_(g) * w);
+            h = h > p.limit ? p.limit : h < -p.limit ? -p.limit : h;
+            reinterpret_cast<__nv_bfloat16*>(p.y)[(int64_t)(x0 + tok + i) * p.ldy + col] = f2bf(siluf_(g) * h);
           }
         } else {
           if (n >= p.N) continue;
           const float sc = !NV || own ? rs : __ldcg(p.row_scale + n);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (tok + i < p.M) store1(p, tok + i, n, vs[i] * sc);
+            if (tok + i < M) store1(p, x0 + tok + i, n, vs[i] * sc);
         }
       }
     }
@@ -557,11 +584,11 @@ static cudaError_t sk_active(int dev, int CL, int* out) {
 }
 
 // the dynamic shared memory limit of a kernel, raised once per device
-template <bool NV, bool WIDE, bool INLINE>
+template <bool NV, int T, bool WIDE, bool INLINE>
 static cudaError_t sk_prepare(int dev) {
   static std::atomic<bool> done[kMaxDev];
   if (dev < kMaxDev && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(fp4_skinny_kernel<NV, WIDE, INLINE>,
+  const cudaError_t e = cudaFuncSetAttribute(fp4_skinny_kernel<NV, T, WIDE, INLINE>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, sk_budget(WIDE));
   if (e == cudaSuccess && dev < kMaxDev) done[dev].store(true, std::memory_order_relaxed);
   return e;
@@ -572,13 +599,18 @@ static cudaError_t sk_prepare(int dev) {
 // more and 0.08 for each row and CTA of the cluster (its reduction is not hidden), the last reduction 0.047.  A cluster
 // launch keeps an eighth of the room free: with all of it in use, a CTA of a neighbouring kernel makes one cluster wait
 // (32 clusters of 8 where 33 fit: 9.5 us, or 15.6).
-template <bool NV, bool WIDE, bool INLINE>
-static cudaError_t sk_plan(int M, int64_t N, int K, int dev, SkPlan& b, double& cost) {
+template <bool NV, int T, bool WIDE, bool INLINE>
+static cudaError_t sk_plan(int M, int64_t N, int K, int group, int dev, SkPlan& b, double& cost) {
   constexpr int kSB = Fmt<NV>::kScaleBytes;
   b = SkPlan{};
-  b.blocks = (int)((N + 127) / 128);
+  b.group = group;
+  b.groups = (M + group - 1) / group;
+  M = std::min(M, group);                             // rows of a group
+  const int64_t units = (N + 127) / 128 * b.groups;
+  if (units >= (int64_t)1 << 31) return cudaErrorInvalidConfiguration;
+  b.units = (int)units;
   b.KT = tiles_k(K);
-  b.ncol = std::max(16, (M * kTerms + 15) / 16 * 16);
+  b.ncol = std::max(16, (M * T + 15) / 16 * 16);
   const int xtile = b.ncol * 128 + (b.ncol > 128 ? 2 : 1) * kSB;
   b.stage_bytes = (kTileBytes + kSB + (INLINE ? 0 : xtile) + 1023) / 1024 * 1024;
   for (int cl = 1; cl <= 8 && cl <= b.KT; ++cl) {
@@ -592,7 +624,7 @@ static cudaError_t sk_plan(int M, int64_t N, int K, int dev, SkPlan& b, double& 
     const int xbytes = INLINE ? (per * xtile + 1023) / 1024 * 1024 : 0;
     const int stages = std::min(8, (sk_budget(WIDE) - 1024 - xbytes - sk_recv_bytes(cl, M)) / b.stage_bytes);
     if (stages < (INLINE ? 4 : 2)) continue;           // a resident expansion must leave the ring its depth
-    const int clusters = std::min(b.blocks, active), rounds = (b.blocks + clusters - 1) / clusters;
+    const int clusters = std::min(b.units, active), rounds = (b.units + clusters - 1) / clusters;
     const double c = rounds * per + (rounds - 1) * (4 + 0.08 * M * cl) + 0.047 * M * cl;
     if (b.CL == 0 || c < cost) {
       cost = c;
@@ -606,16 +638,26 @@ static cudaError_t sk_plan(int M, int64_t N, int K, int dev, SkPlan& b, double& 
   return b.CL ? cudaSuccess : cudaErrorInvalidConfiguration;
 }
 
-template <bool NV, bool WIDE, bool INLINE>
+template <bool NV, int T, bool WIDE, bool INLINE>
 static cudaError_t launch_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   SkPlan b;
-  double cost;
-  if (e == cudaSuccess) e = sk_prepare<NV, WIDE, INLINE>(dev);
-  if (e == cudaSuccess) e = sk_plan<NV, WIDE, INLINE>(p.M, p.N, p.K, dev, b, cost);
+  double cost = 0;
+  if (e == cudaSuccess) e = sk_prepare<NV, T, WIDE, INLINE>(dev);
+  if (T > 1) {
+    if (e == cudaSuccess) e = sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, WIDE ? 32 : 16, dev, b, cost);
+  } else {
+    // 4-bit rows: 128 at a time read W fewer times, 64 leave room for the exchange of a cluster
+    SkPlan c;
+    double wide_cost = 0;
+    if (e == cudaSuccess) e = sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, 64, dev, b, cost);
+    if (e == cudaSuccess && p.M > 64 &&
+        sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, 128, dev, c, wide_cost) == cudaSuccess && wide_cost < cost)
+      b = c;
+  }
   if (e != cudaSuccess) return e;
-  const int smem = b.xbytes + b.stages * b.stage_bytes + sk_recv_bytes(b.CL, p.M) + 1024;
+  const int smem = b.xbytes + b.stages * b.stage_bytes + sk_recv_bytes(b.CL, std::min(p.M, b.group)) + 1024;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(b.clusters * b.CL);
   cfg.blockDim = dim3(kSkThreads);
@@ -637,7 +679,7 @@ static cudaError_t launch_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
   }
   cfg.attrs = at;
   cfg.numAttrs = na;
-  return cudaLaunchKernelEx(&cfg, fp4_skinny_kernel<NV, WIDE, INLINE>, p, b);
+  return cudaLaunchKernelEx(&cfg, fp4_skinny_kernel<NV, T, WIDE, INLINE>, p, b);
 }
 
 // a launch of fp4_expand costs about 3 tiles, so a plan with the expansion in the kernel may be that much worse
@@ -647,14 +689,15 @@ static bool expand_inline_t(int M, int64_t N, int K) {
   SkPlan b;
   double in = 0, sep = 0;
   return M <= 8 && cudaGetDevice(&dev) == cudaSuccess &&
-         sk_plan<NV, false, true>(M, N, K, dev, b, in) == cudaSuccess &&
-         sk_plan<NV, false, false>(M, N, K, dev, b, sep) == cudaSuccess && in <= sep + 3;
+         sk_plan<NV, kTerms, false, true>(M, N, K, 16, dev, b, in) == cudaSuccess &&
+         sk_plan<NV, kTerms, false, false>(M, N, K, 16, dev, b, sep) == cudaSuccess && in <= sep + 3;
 }
 
 template <bool NV>
 static cudaError_t skinny_t(const Fp4SkinnyArgs& p, cudaStream_t st) {
-  if (p.x) return launch_skinny<NV, false, true>(p, st);
-  return p.M <= 16 ? launch_skinny<NV, false, false>(p, st) : launch_skinny<NV, true, false>(p, st);
+  if (p.x) return launch_skinny<NV, kTerms, false, true>(p, st);
+  if (p.terms == 1) return launch_skinny<NV, 1, true, false>(p, st);
+  return p.M <= 16 ? launch_skinny<NV, kTerms, false, false>(p, st) : launch_skinny<NV, kTerms, true, false>(p, st);
 }
 
 }  // namespace fp4
@@ -669,14 +712,14 @@ bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv) {
 }
 
 cudaError_t g53_fp4_expand(const Fp4ExpandArgs& p, cudaStream_t st) {
-  if (p.M < 1 || p.M > 32 || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
+  if (p.M < 1 || p.M > 65535 || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
   const dim3 grid((fp4::tiles_k(p.K) * 32 + 255) / 256, p.M);
   return p.nv ? g53_launch_pdl(fp4::fp4_expand_kernel<true>, grid, dim3(256), 0, st, 1, p)
               : g53_launch_pdl(fp4::fp4_expand_kernel<false>, grid, dim3(256), 0, st, 1, p);
 }
 
 cudaError_t g53_fp4_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
-  if (p.M < 1 || p.M > 32 || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
+  if (p.M < 1 || p.N < 1 || (p.x && p.M > 8) || p.K < 16 || p.K % (p.nv ? 16 : 32)) return cudaErrorInvalidValue;
   return p.nv ? fp4::skinny_t<true>(p, st) : fp4::skinny_t<false>(p, st);
 }
 

@@ -596,7 +596,7 @@ cudaError_t g53_gemm_sm100(const GemmArgs& p, cudaStream_t st) {
     return cudaErrorInvalidValue;
   if (p.batch > 1 && (((p.bsa * esz) & 15) || ((p.bsb * esz) & 15) || p.a_scale)) return cudaErrorInvalidValue;
   if (p.fp8) return p.N >= 256 ? launch<256, true, 4>(p, st) : launch<128, true, 6>(p, st);
-  return p.N >= 256 ? launch<256, false, 4>(p, st) : launch<128, false, 6>(p, st);
+  return p.N >= 256 && p.bn != 128 ? launch<256, false, 4>(p, st) : launch<128, false, 6>(p, st);
 }
 
 cudaError_t g53_quant_rows_e4m3(const __nv_bfloat16* x, int64_t ldx, int R, int K, uint8_t* q, float* scale,

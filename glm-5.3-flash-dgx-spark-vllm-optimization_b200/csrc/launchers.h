@@ -68,6 +68,7 @@ struct GemmArgs {
   float limit;
   int* err;                            // device error word (bounded waits that ran out)
   int vec;                             // set by the launcher: 16-byte epilogue stores allowed
+  int bn;                              // bf16: 128 = tiles of 128 columns even for N >= 256 (0: by N)
   // batched GEMM (e.g. per attention head): batch strides in elements of A, B, Y and of b_scale
   int batch;                           // 0 or 1: a single GEMM
   int64_t bsa, bsb, bsy, bss;
@@ -413,7 +414,7 @@ struct Fp4DequantArgs {
 };
 cudaError_t g53_fp4_dequant(const Fp4DequantArgs& p, cudaStream_t st);
 
-// Expansion of M <= 32 bf16 rows into g53_fp4_terms() 4-bit rows each (fp4_skinny.cu): image rows terms * m + t
+// Expansion of M bf16 rows into g53_fp4_terms() 4-bit rows each (fp4_skinny.cu): image rows terms * m + t
 int g53_fp4_terms();
 // whether the product expands these rows itself, without a launch of g53_fp4_expand
 bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv);
@@ -426,11 +427,13 @@ struct Fp4ExpandArgs {
 };
 cudaError_t g53_fp4_expand(const Fp4ExpandArgs& p, cudaStream_t st);
 
-// y[M, N] (mode) = x[M, K] @ W4[N, K]^T for M <= 32 (fp4_skinny.cu), x as rows or expanded.  GEMV_SWIGLU: W4 is a gate/up image
+// y[M, N] (mode) = x[M, K] @ W4[N, K]^T for few rows (fp4_skinny.cu), x as rows, expanded, or 4-bit rows.  GEMV_SWIGLU: W4 is a gate/up image
 // (64 gate rows, then their 64 up rows, per 128-row block), y [M, width] bf16
 struct Fp4SkinnyArgs {
   const __nv_bfloat16* x; int64_t ldx; int xvec;   // the rows themselves (expanded by the kernel), or null:
   const uint8_t* x_codes; const uint8_t* x_scales; const float* x_factor;
+  float x_const;                       // factor of every row where x_factor is null
+  int terms;                           // 4-bit rows per row of x: g53_fp4_terms() or 1 (x_factor: the row scales)
   const uint8_t* codes; const uint8_t* scales; const float* row_scale;
   int nv;
   void* y; int64_t ldy;

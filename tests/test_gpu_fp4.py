@@ -210,7 +210,7 @@ def test_linear_reads_nan_weights_as_nan(fmt):
     w = weight(256, 512, 3)
     w[10, 20] = math.nan
     w4 = fp4.quantize4(w, fmt)
-    for m, act4 in ((3, False), (40, True), (70, False)):
+    for m, act4 in ((3, False), (40, True), (70, False), (150, True), (270, False)):
         y = fp4.linear4(acts(m, 512, m), w4, torch.empty(m, 256, dtype=F32, device="cuda"), K.GEMV_F32, act4=act4)
         bad = torch.zeros(256, dtype=torch.bool, device="cuda")
         bad[10] = True
@@ -218,7 +218,7 @@ def test_linear_reads_nan_weights_as_nan(fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("m", [17, 40, 63, 64, 200])
+@pytest.mark.parametrize("m", [17, 40, 63, 64, 200, 256, 257, 300])
 def test_linear_exact_activations_above_16_rows(fmt, m):
     n, k = 300, 800
     x, w = acts(m, k, m), weight(n, k, 5)
@@ -238,7 +238,7 @@ def test_linear_exact_activations_above_16_rows(fmt, m):
 
 # ------------------------------------------------------------------------------------- linear, 4-bit activations
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("m,n,k", [(17, 8, 32), (64, 128, 64), (100, 100, 96), (128, 256, 256), (129, 257, 288),
+@pytest.mark.parametrize("m,n,k", [(17, 8, 32), (64, 128, 64), (100, 100, 96), (65, 20000, 96), (128, 200, 4128), (127, 4096, 96), (128, 256, 256), (129, 257, 288),
                                    (300, 1000, 1536), (70, 130, 4128), (1000, 520, 320), (2500, 4100, 544),
                                    (4096, 2048, 1024), (2433, 2817, 96), (129, 19100, 288)])
 def test_linear_4bit_activations(fmt, m, n, k):
@@ -309,7 +309,8 @@ def h_slack(h, err, fmt, bound):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,k,width,n", [(1, 4096, 2048, 512), (8, 512, 96, 40), (16, 288, 1536, 200), (5, 64, 32, 1),
-                                         (33, 256, 160, 128), (64, 512, 96, 40), (150, 256, 1536, 200)])
+                                         (33, 256, 160, 128), (64, 512, 96, 40), (150, 256, 1536, 200), (257, 512, 96, 40),
+                                         (300, 256, 1536, 200)])
 def test_mlp_exact_activations(fmt, m, k, width, n):
     limit = 2.0
     x, gate, up, down = acts(m, k, m), weight(width, k, 1), weight(width, k, 2), weight(n, width, 3)
@@ -359,7 +360,7 @@ def test_mlp_4bit_activations(fmt, m, k, width, n):
 @pytest.mark.parametrize("fmt", FMTS)
 def test_mlp_keeps_a_nan_row(fmt):
     mlp = fp4.pack_mlp4(weight(96, 256, 1), weight(96, 256, 2), weight(64, 96, 3), fmt)
-    for m, act4 in ((4, False), (40, True), (40, False), (80, False)):
+    for m, act4 in ((4, False), (40, True), (140, True), (40, False), (80, False), (270, False)):
         x = acts(m, 256, m)
         x[2, 17] = math.nan
         y = fp4.mlp4(x, mlp, torch.empty(m, 64, dtype=F32, device="cuda"), 10.0, act4=act4)
@@ -376,7 +377,8 @@ def test_mlp_without_a_clamp():
 
 
 # ---------------------------------------------------------------------------------------- graphs, streams, reuse
-@pytest.mark.parametrize("m,act4", [(3, False), (12, False), (30, False), (90, False), (90, True)])
+@pytest.mark.parametrize("m,act4", [(3, False), (12, False), (30, False), (90, False), (90, True),
+                                    (200, True), (270, False)])
 def test_graph_replay_and_streams(m, act4):
     """Quantise, project and run the block as one captured graph, replayed on new inputs, beside eager calls on another
     stream: all the same bits."""
