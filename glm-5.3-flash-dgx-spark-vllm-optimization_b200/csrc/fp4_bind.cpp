@@ -193,7 +193,7 @@ void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t width, i
   const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
   const int vec = aligned16(rows) && x.stride(0) % 8 == 0;
   Tensor buf;
-  if (g53_fp4_expand_inline(a.M, a.N, a.K, a.nv)) {
+  if (g53_fp4_expand_inline(a.M, a.N, a.K, a.nv, mode == GEMV_SWIGLU)) {
     a.x = rows;
     a.ldx = x.stride(0);
     a.xvec = vec;

@@ -548,7 +548,9 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
 
 constexpr int kMaxDev = 64;
 
-static int sk_recv_bytes(int CL, int M) { return 2 * CL * ((M + 3) & ~3) * 2 * ((64 + CL - 1) / CL) * 4; }
+static int sk_recv_bytes(int CL, int M, bool swi) {
+  return CL == 1 && !swi ? 0 : 2 * CL * ((M + 3) & ~3) * 2 * ((64 + CL - 1) / CL) * 4;
+}
 static int sk_budget(bool wide) { return (wide ? 225 : 111) * 1024; }
 
 // Stands in for the product in the question below: the runtime answers one CTA per SM for any kernel that uses TMEM
@@ -600,7 +602,7 @@ static cudaError_t sk_prepare(int dev) {
 // launch keeps an eighth of the room free: with all of it in use, a CTA of a neighbouring kernel makes one cluster wait
 // (32 clusters of 8 where 33 fit: 9.5 us, or 15.6).
 template <bool NV, int T, bool WIDE, bool INLINE>
-static cudaError_t sk_plan(int M, int64_t N, int K, int group, int dev, SkPlan& b, double& cost) {
+static cudaError_t sk_plan(int M, int64_t N, int K, int group, bool swi, int dev, SkPlan& b, double& cost) {
   constexpr int kSB = Fmt<NV>::kScaleBytes;
   b = SkPlan{};
   b.group = group;
@@ -611,7 +613,7 @@ static cudaError_t sk_plan(int M, int64_t N, int K, int group, int dev, SkPlan& 
   b.units = (int)units;
   b.KT = tiles_k(K);
   b.ncol = std::max(16, (M * T + 15) / 16 * 16);
-  const int xtile = b.ncol * 128 + (b.ncol > 128 ? 2 : 1) * kSB;
+  const int xtile = b.ncol * 128 + (WIDE && T > 1 ? 2 : 1) * kSB;
   b.stage_bytes = (kTileBytes + kSB + (INLINE ? 0 : xtile) + 1023) / 1024 * 1024;
   for (int cl = 1; cl <= 8 && cl <= b.KT; ++cl) {
     const int per = (b.KT + cl - 1) / cl;
@@ -622,7 +624,7 @@ static cudaError_t sk_plan(int M, int64_t N, int K, int group, int dev, SkPlan& 
     if (e != cudaSuccess) return e;
     if (cl > 1) active -= active / 8;
     const int xbytes = INLINE ? (per * xtile + 1023) / 1024 * 1024 : 0;
-    const int stages = std::min(8, (sk_budget(WIDE) - 1024 - xbytes - sk_recv_bytes(cl, M)) / b.stage_bytes);
+    const int stages = std::min(8, (sk_budget(WIDE) - 1024 - xbytes - sk_recv_bytes(cl, M, swi)) / b.stage_bytes);
     if (stages < (INLINE ? 4 : 2)) continue;           // a resident expansion must leave the ring its depth
     const int clusters = std::min(b.units, active), rounds = (b.units + clusters - 1) / clusters;
     const double c = rounds * per + (rounds - 1) * (4 + 0.08 * M * cl) + 0.047 * M * cl;
@@ -644,20 +646,21 @@ static cudaError_t launch_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   SkPlan b;
   double cost = 0;
+  const bool swi = p.mode == GEMV_SWIGLU;
   if (e == cudaSuccess) e = sk_prepare<NV, T, WIDE, INLINE>(dev);
   if (T > 1) {
-    if (e == cudaSuccess) e = sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, WIDE ? 32 : 16, dev, b, cost);
+    if (e == cudaSuccess) e = sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, WIDE ? 32 : 16, swi, dev, b, cost);
   } else {
     // 4-bit rows: 128 at a time read W fewer times, 64 leave room for the exchange of a cluster
     SkPlan c;
     double wide_cost = 0;
-    if (e == cudaSuccess) e = sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, 64, dev, b, cost);
+    if (e == cudaSuccess) e = sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, 64, swi, dev, b, cost);
     if (e == cudaSuccess && p.M > 64 &&
-        sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, 128, dev, c, wide_cost) == cudaSuccess && wide_cost < cost)
+        sk_plan<NV, T, WIDE, INLINE>(p.M, p.N, p.K, 128, swi, dev, c, wide_cost) == cudaSuccess && wide_cost < cost)
       b = c;
   }
   if (e != cudaSuccess) return e;
-  const int smem = b.xbytes + b.stages * b.stage_bytes + sk_recv_bytes(b.CL, std::min(p.M, b.group)) + 1024;
+  const int smem = b.xbytes + b.stages * b.stage_bytes + sk_recv_bytes(b.CL, std::min(p.M, b.group), swi) + 1024;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(b.clusters * b.CL);
   cfg.blockDim = dim3(kSkThreads);
@@ -684,13 +687,13 @@ static cudaError_t launch_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
 
 // a launch of fp4_expand costs about 3 tiles, so a plan with the expansion in the kernel may be that much worse
 template <bool NV>
-static bool expand_inline_t(int M, int64_t N, int K) {
+static bool expand_inline_t(int M, int64_t N, int K, bool swi) {
   int dev = 0;
   SkPlan b;
   double in = 0, sep = 0;
   return M <= 8 && cudaGetDevice(&dev) == cudaSuccess &&
-         sk_plan<NV, kTerms, false, true>(M, N, K, 16, dev, b, in) == cudaSuccess &&
-         sk_plan<NV, kTerms, false, false>(M, N, K, 16, dev, b, sep) == cudaSuccess && in <= sep + 3;
+         sk_plan<NV, kTerms, false, true>(M, N, K, 16, swi, dev, b, in) == cudaSuccess &&
+         sk_plan<NV, kTerms, false, false>(M, N, K, 16, swi, dev, b, sep) == cudaSuccess && in <= sep + 3;
 }
 
 template <bool NV>
@@ -707,8 +710,8 @@ using namespace g53;
 
 int g53_fp4_terms() { return fp4::kTerms; }
 
-bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv) {
-  return nv ? fp4::expand_inline_t<true>(M, N, K) : fp4::expand_inline_t<false>(M, N, K);
+bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv, bool swiglu) {
+  return nv ? fp4::expand_inline_t<true>(M, N, K, swiglu) : fp4::expand_inline_t<false>(M, N, K, swiglu);
 }
 
 cudaError_t g53_fp4_expand(const Fp4ExpandArgs& p, cudaStream_t st) {

@@ -417,7 +417,7 @@ cudaError_t g53_fp4_dequant(const Fp4DequantArgs& p, cudaStream_t st);
 // Expansion of M bf16 rows into g53_fp4_terms() 4-bit rows each (fp4_skinny.cu): image rows terms * m + t
 int g53_fp4_terms();
 // whether the product expands these rows itself, without a launch of g53_fp4_expand
-bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv);
+bool g53_fp4_expand_inline(int M, int64_t N, int K, int nv, bool swiglu);
 struct Fp4ExpandArgs {
   const __nv_bfloat16* x; int64_t ldx;
   int M, K, nv;
