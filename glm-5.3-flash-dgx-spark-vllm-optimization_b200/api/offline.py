@@ -41,6 +41,8 @@ class LLMOptions:
     block_verify: bool = False          # sampled requests: block verification instead of standard
     mixed_prefill_chunk: int = 0        # prefill tokens per step while requests decode (0: the whole chunk)
     ep: bool = False                    # routed experts expert-parallel over the ranks (parallel/ep.py)
+    mlp4: str | None = None             # dense MLPs and shared experts in 4 bits: "nvfp4" or "mxfp4" (one GPU)
+    mlp4_act4: bool = False             # with mlp4: 4-bit activations, too, in prefill chunks
     sp_mla: bool = os.environ.get("GLM53_SP_MLA", "1") == "1"   # row-parallel MLA in sequence-parallel prefill
 
 
@@ -68,7 +70,8 @@ class LLM:
             src = W.OverrideSource(src, opts.overrides, opts.override_sha256)
         self.cfg: ModelConfig = cfg
         t0 = time.time()
-        self.weights = W.prepare(src, cfg, rank=rank, world=world, device=dev, ep=opts.ep, sp_mla=opts.sp_mla)
+        self.weights = W.prepare(src, cfg, rank=rank, world=world, device=dev, ep=opts.ep, sp_mla=opts.sp_mla,
+                                 mlp4=opts.mlp4)
         self.load_s = time.time() - t0
         if opts.kv_cache_bytes and not opts.kv_pages:
             opts.kv_pages = max(1, int(opts.kv_cache_bytes // (cfg.kv_bytes_per_token() * opts.page_size)))
@@ -79,7 +82,7 @@ class LLM:
                            kv_slots=pages * opts.page_size, block_size=opts.page_size,
                            max_blocks=(opts.max_model_len + opts.page_size - 1) // opts.page_size + 2,
                            decode_rows=max(16, opts.max_seqs * (kmax + 1)),
-                           logit_rows=max(16, opts.max_seqs * (kmax + 1)))
+                           logit_rows=max(16, opts.max_seqs * (kmax + 1)), mlp4_act4=opts.mlp4_act4)
         self.backend = GPUBackend(self.weights, rc, comm=comm, drafter=opts.speculative,
                                   cuda_graphs=opts.cuda_graphs, checkpoints=opts.checkpoints)
         ec = EngineConfig(max_seqs=opts.max_seqs, page_size=opts.page_size, num_pages=pages,

@@ -512,6 +512,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--block-verify", action="store_true", help="block verification for sampled requests")
     ap.add_argument("--vtrim-tau", type=float, default=0.0, help="verify trimming by drafter confidence (0: off)")
     ap.add_argument("--no-cuda-graphs", action="store_true")
+    ap.add_argument("--mlp4", choices=["nvfp4", "mxfp4"], default=None,
+                    help="dense MLPs and shared experts in 4 bits (one GPU)")
+    ap.add_argument("--mlp4-act4", action="store_true", help="with --mlp4: 4-bit activations in prefill chunks, too")
     ap.add_argument("--served-model-name", default="glm-5.3-flash")
     ap.add_argument("--api-key", default=None, help="require Authorization: Bearer <key> on /v1 routes")
     ap.add_argument("--no-reasoning-parser", action="store_true")
@@ -526,7 +529,8 @@ def options_from_args(args):
                       page_size=args.page_size, kv_cache_bytes=args.kv_cache_bytes, checkpoints=args.checkpoints,
                       speculative=not args.no_spec, k_set=tuple(int(k) for k in args.k_set.split(",")),
                       k_fixed=args.num_speculative_tokens, block_verify=args.block_verify,
-                      vtrim_tau=args.vtrim_tau, cuda_graphs=not args.no_cuda_graphs)
+                      vtrim_tau=args.vtrim_tau, cuda_graphs=not args.no_cuda_graphs, mlp4=args.mlp4,
+                      mlp4_act4=args.mlp4_act4)
 
 
 def serve(argv=None):

@@ -24,6 +24,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
+from ..ops import fp4
 from ..ops import kernels as K
 from ..utils.canary import Scratch
 from .weights import Linear8, Weights
@@ -46,6 +47,7 @@ class RuntimeConfig:
     moe_prefill_rows: int = 8192  # rows per routed-MoE launch group of the prefill (tcgen05) path
     attn_chunk: int = 1024        # rows per attention launch group (scratch bound)
     logit_rows: int = 16
+    mlp4_act4: bool = False       # 4-bit MLPs: activations in 4 bits too, in forwards of more than decode_rows rows
 
 
 def interleave_gate_up(gu: Linear8) -> Linear8:
@@ -133,7 +135,8 @@ class Runtime:
         self.gu_il = {}
         for lw in w.layers:
             m = lw.mlp if lw.mlp is not None else lw.moe.shared
-            self.gu_il[lw.index] = interleave_gate_up(m.gu)
+            if m.four is None:
+                self.gu_il[lw.index] = interleave_gate_up(m.gu)
         # scratch: guard bands around every buffer in the bounds-checked build (utils/canary.py)
         self.scratch = Scratch(dev)
         self.scratch.attach(self)
@@ -230,7 +233,7 @@ class Runtime:
         tk = c.top_k
         P = MR * tk
         widths = [self.gu_il[i].w.shape[0] // 2 for i in self.gu_il]
-        self.act = z(R, max(widths), dtype=bf16, device=dev)
+        self.act = z(R, max(widths, default=1), dtype=bf16, device=dev)
         self.rlogits = z(MR, c.experts, dtype=f32, device=dev)
         self.topk_ids = z(MR, tk, dtype=i32, device=dev)
         self.topk_w = z(MR, tk, dtype=f32, device=dev)
@@ -639,8 +642,16 @@ class Runtime:
         K.linear8(self.o_lat[:R].transpose(0, 1), a.w_uv.w, a.w_uv.s, ob.transpose(0, 1))
         self._final_linear(self.obuf[:R], a.o_proj, R, proj="mla_o_proj")
 
+    def _mlp4(self, m, R, mode):
+        """A 4-bit MLP block into the branch (its temporaries come from the allocator's pool of the current stream)."""
+        fp4.mlp4(self.normed[:R], m, self.branch[:R], self.cfg.limit, mode,
+                 act4=self.rc.mlp4_act4 and R > self.rc.decode_rows)
+
     def _mlp(self, lw, R):
         m = lw.mlp
+        if m.four is not None:
+            self._mlp4(m.four, R, K.GEMV_F32)
+            return
         gu = self.gu_il[lw.index]
         act = self.act[:R, :m.width]
         K.linear8(self.normed[:R], gu.w, gu.s, act, K.GEMV_SWIGLU, self.cfg.limit)
@@ -699,10 +710,13 @@ class Runtime:
             self.ev_fork.record()
             with torch.cuda.stream(self.side):
                 self.side.wait_event(self.ev_fork)
-                act = self.act[:R, :s.width]
-                K.linear8(self.normed[:R], self.gu_il[lw.index].w, self.gu_il[lw.index].s, act, K.GEMV_SWIGLU,
-                          c.limit)
-                K.linear8(act, s.down.w, s.down.s, self.branch[:R], K.GEMV_F32)
+                if s.four is not None:
+                    self._mlp4(s.four, R, K.GEMV_F32)
+                else:
+                    act = self.act[:R, :s.width]
+                    K.linear8(self.normed[:R], self.gu_il[lw.index].w, self.gu_il[lw.index].s, act, K.GEMV_SWIGLU,
+                              c.limit)
+                    K.linear8(act, s.down.w, s.down.s, self.branch[:R], K.GEMV_F32)
                 self.ev_join.record()
             P = R * c.top_k
             x = self.normed[:R]
@@ -739,9 +753,12 @@ class Runtime:
         self._shared_expert(lw, R)
 
     def _shared_expert(self, lw, R):
-        """The shared expert (fp8 SwiGLU MLP), accumulated into the branch."""
+        """The shared expert (fp8 or 4-bit SwiGLU MLP), accumulated into the branch."""
         c, m = self.cfg, lw.moe
         s = m.shared
+        if s.four is not None:
+            self._mlp4(s.four, R, K.GEMV_F32_ACC)
+            return
         gu = self.gu_il[lw.index]
         act = self.act[:R, :s.width]
         K.linear8(self.normed[:R], gu.w, gu.s, act, K.GEMV_SWIGLU, c.limit)

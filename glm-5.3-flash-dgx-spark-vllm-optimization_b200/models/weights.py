@@ -34,6 +34,7 @@ import torch
 
 from ..config import ModelConfig
 from ..ops import exl3 as exl3_ops
+from ..ops import fp4 as fp4_ops
 
 P = "model."
 FP8_MAX = 448.0
@@ -138,9 +139,10 @@ class MLAFull:
 
 @dataclass
 class MLPW:
-    gu: Linear8               # [2*Wl, D]  (gate rows then up rows)
-    down: Linear8             # [D, Wl]
+    gu: Linear8 | None        # [2*Wl, D]  (gate rows then up rows)
+    down: Linear8 | None      # [D, Wl]
     width: int
+    four: fp4_ops.MLP4 | None = None     # the block in 4 bits, in place of gu and down (prepare(mlp4=...))
 
 
 @dataclass
@@ -198,6 +200,8 @@ class Weights:
             elif hasattr(o, "__dataclass_fields__"):
                 for k in o.__dataclass_fields__:
                     add(getattr(o, k))
+            elif isinstance(o, fp4_ops.Matrix4):
+                total += o.nbytes
         add(self.embed)
         add(self.layers)
         add(self.norm)
@@ -529,11 +533,21 @@ def _rows(x: torch.Tensor, rank: int, world: int, dim: int = 0) -> torch.Tensor:
 
 def prepare(src: TensorSource, cfg: ModelConfig, *, rank: int = 0, world: int = 1,
             device: str | torch.device = "cpu", layers: list[int] | None = None,
-            progress: Callable[[str], None] | None = None, ep: bool = False, sp_mla: bool = False) -> Weights:
+            progress: Callable[[str], None] | None = None, ep: bool = False, sp_mla: bool = False,
+            mlp4: str | None = None) -> Weights:
     """Quantise and shard a checkpoint into runtime weights for rank ``rank`` of ``world``.  ``ep``: the routed
     experts are sharded by expert (rank j holds experts [j E/W, (j+1) E/W) at full width, for the expert-parallel
     MoE of parallel/ep.py) instead of by width; everything else stays tensor-parallel.  ``sp_mla``: the MLA
-    layers also keep every head's query / output projections (``MLAW.full``) for row-parallel prefill."""
+    layers also keep every head's query / output projections (``MLAW.full``) for row-parallel prefill.  ``mlp4``
+    ("nvfp4" or "mxfp4"): the dense MLPs and shared experts in 4 bits instead of fp8 (ops/fp4.py; one GPU, their widths
+    multiples of 32)."""
+    if mlp4 is not None:
+        if mlp4 not in fp4_ops.FORMATS:
+            raise ValueError(f"mlp4 must be one of {', '.join(fp4_ops.FORMATS)}, got {mlp4!r}")
+        if world > 1:
+            raise ValueError("4-bit MLPs are not sharded: mlp4 needs world == 1")
+        if torch.device(device).type != "cuda":
+            raise ValueError("4-bit MLPs are quantised on the GPU: mlp4 needs a CUDA device")
     if ep and world > 1 and cfg.experts % world:
         raise ValueError(f"{cfg.experts} experts do not split over {world} ranks")
     c = cfg
@@ -607,6 +621,9 @@ def prepare(src: TensorSource, cfg: ModelConfig, *, rank: int = 0, world: int = 
     def mlp(prefix, width):
         gate = _rows(g(prefix + "gate_proj.weight"), rank, world).to(dev)
         up = _rows(g(prefix + "up_proj.weight"), rank, world).to(dev)
+        if mlp4 is not None:
+            down = g(prefix + "down_proj.weight").to(dev)
+            return MLPW(None, None, width, fp4_ops.pack_mlp4(bf(gate), bf(up), bf(down), mlp4))
         return MLPW(lin(torch.cat([gate, up], 0)), lin_rowpar(g(prefix + "down_proj.weight")), width // world)
 
     def experts(i, proj):

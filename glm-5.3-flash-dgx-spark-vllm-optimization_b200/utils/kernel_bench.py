@@ -3,7 +3,7 @@ CUDA events after warm-up (an L2 flush -- a 256 MB write -- between timed iterat
 the time and the achieved rate against the measured peaks (MEASURED_PEAKS.json when present).
 
   python -m glm53.utils.kernel_bench moe --tokens 1 8 64 512 8192 [--tp 1]      (BASELINE configs[1])
-  python -m glm53.utils.kernel_bench gemv|gemm|kda|mla|all
+  python -m glm53.utils.kernel_bench gemv|gemm|kda|mla|fp4|all
   torchrun --nproc-per-node N -m glm53.utils.kernel_bench ag --rows 1024 4096    (fused all-gather + GEMM vs NCCL)
   torchrun --nproc-per-node N -m glm53.utils.kernel_bench ep --tokens 1 8 64 512   (experts
       EP-sharded over N GPUs, tokens per rank; dispatch/combine fused into the kernels)
@@ -213,6 +213,34 @@ def bench_gemm(args, T: Timer):
         fl = 2.0 * M * N * Kd
         emit({"case": "gemm_tcgen05", "M": M, "N": N, "K": Kd, "ms_w8a16": ms, "ms_bf16_only": ms_bf,
               "tflops": fl / ms_bf / 1e9, "frac_of_bf16_peak": fl / ms_bf / 1e9 / tflops})
+
+
+def bench_fp4(args, T: Timer):
+    """The 4-bit operators at --tokens rows: quantise, the dense layers' gate/up projection and MLP block (exact and, above
+    16 rows, 4-bit activations), against HBM up to 16 rows and four times the bf16 peak above."""
+    from glm53.ops import fp4
+    from glm53.ops import kernels as K
+    hbm, tflops = peaks()
+    D, W = 4096, 12288
+    for fmt in fp4.FORMATS:
+        gate, up = ((torch.randn(W, D, device="cuda") / 64).to(torch.bfloat16) for _ in range(2))
+        down = (torch.randn(D, W, device="cuda") / 110).to(torch.bfloat16)
+        mlp = fp4.pack_mlp4(gate, up, down, fmt)
+        for m in args.tokens:
+            x = torch.randn(m, D, device="cuda").to(torch.bfloat16)
+            y, g = (torch.empty(m, n, device="cuda", dtype=torch.float32) for n in (D, mlp.gu.rows))
+            ms = T(lambda: fp4.quantize4(x, fmt))
+            emit({"case": "fp4_quantize", "fmt": fmt, "rows": m, "K": D, "ms": ms,
+                  "gbs": (2 * m * D + (m * D * 9) // 16) / ms / 1e6})
+            for act4 in ((False, True) if m > 16 else (False,)):
+                for name, run, nbytes, flops in (
+                        ("fp4_linear", lambda: fp4.linear4(x, mlp.gu, g, K.GEMV_F32, act4=act4), mlp.gu.nbytes,
+                         2.0 * m * D * mlp.gu.rows),
+                        ("fp4_mlp", lambda: fp4.mlp4(x, mlp, y, 10.0, act4=act4), mlp.nbytes, 6.0 * m * D * W)):
+                    ms = T(run)
+                    emit({"case": name, "fmt": fmt, "rows": m, "act4": act4, "ms": ms, "gbs": nbytes / ms / 1e6,
+                          "tflops": flops / ms / 1e9, "frac_of_measured": nbytes / ms / 1e6 / hbm if m <= 16
+                          else flops / ms / 1e9 / (4 * tflops)})
 
 
 def bench_kda(args, T: Timer):
@@ -475,7 +503,7 @@ def bench_dsa(args, T: Timer):
 
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["moe", "gemv", "gemm", "kda", "mla", "ep", "hc", "ag", "dsa", "all"])
+    ap.add_argument("case", choices=["moe", "gemv", "gemm", "kda", "mla", "ep", "hc", "ag", "dsa", "fp4", "all"])
     ap.add_argument("--tokens", type=int, nargs="+", default=[1, 8, 64, 512, 8192])
     ap.add_argument("--rows", type=int, nargs="+", default=[8])
     ap.add_argument("--kda-rows", type=int, nargs="+", default=[8, 8192])

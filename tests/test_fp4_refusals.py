@@ -27,3 +27,22 @@ def u8(n):
 def test_refused(call, words):
     with pytest.raises((RuntimeError, ValueError), match=words):
         call()
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(mlp4="fp4"), "must be one of nvfp4, mxfp4"),
+    (dict(mlp4="nvfp4", world=2), "world == 1"),
+    (dict(mlp4="nvfp4"), "needs a CUDA device"),
+])
+def test_prepare_refuses(tiny_cfg, tiny_ckpt, kw, words):
+    from glm53.models import weights as W
+    with pytest.raises(ValueError, match=words):
+        W.prepare(W.DictSource(tiny_ckpt), tiny_cfg, **kw)
+
+
+def test_server_flags_reach_the_options():
+    from glm53.api.server import build_parser, options_from_args
+    o = options_from_args(build_parser().parse_args(["--mlp4", "mxfp4", "--mlp4-act4"]))
+    assert o.mlp4 == "mxfp4" and o.mlp4_act4
+    o = options_from_args(build_parser().parse_args([]))
+    assert o.mlp4 is None and not o.mlp4_act4

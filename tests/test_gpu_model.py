@@ -129,3 +129,117 @@ def test_tiny_model_chunked_prefill_matches_stepwise(dense_setup):
         seq.commit(1)
     cos, mx = _close(a, b[0])
     assert cos > 0.9995, (cos, mx)
+
+
+class _Dequantised:
+    """Dense weights where the oracle reads the codes and row scales of a Linear8."""
+
+    def __init__(self, w):
+        self.w, self.dense, self.s = self, w.float().cpu(), torch.ones(w.shape[0])
+
+    def view(self, dtype):
+        return self.dense
+
+
+def _oracle_mlp4(w, ckpt, fmt):
+    """The fp32 oracle's weights with every dense MLP replaced by the values of its 4-bit form."""
+    import copy
+    from glm53.models import weights as W
+    from glm53.ops import fp4
+
+    def values(t):
+        return fp4.dequantize4(fp4.quantize4(t.to(torch.bfloat16).to(DEV), fmt), torch.float32).cpu()
+
+    w = copy.copy(w)
+    w.layers = [copy.copy(lw) for lw in w.layers]
+    for lw in w.layers:
+        p = f"model.layers.{lw.index}.mlp."
+        gate, up, down = (values(ckpt[p + n + "_proj.weight"]) for n in ("gate", "up", "down"))
+        lw.mlp = W.MLPW(_Dequantised(torch.cat([gate, up])), _Dequantised(down), gate.shape[0])
+    return w
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_tiny_model_mlp4(fmt):
+    """Dense MLPs in 4 bits in every layer (no expert choice that a rounding could flip): prefill in 64-row chunks and greedy
+    decode against the oracle with the same 4-bit values."""
+    import glm53
+    from glm53.models import weights as W
+    from glm53.models.runtime import Runtime, RuntimeConfig
+    from glm53.models.session import Sequence
+    cfg = dataclasses.replace(glm53.tiny_config(), index_topk=256, mlp_kinds=["dense"] * 4)
+    ckpt = W.random_checkpoint(cfg, seed=0)
+    w4 = W.prepare(W.DictSource(ckpt), cfg, device=DEV, mlp4=fmt)
+    assert w4.layers[0].mlp.gu is None and w4.layers[0].mlp.four.gu.fmt == fmt
+    w8 = W.prepare(W.DictSource(ckpt), cfg)
+    assert w4.nbytes() < w8.nbytes()
+    prompt, toks, ref_logits = _oracle(cfg, _oracle_mlp4(w8, ckpt, fmt))
+    for act4 in (False, True):
+        rt = Runtime(w4, RuntimeConfig(max_rows=64, kv_slots=1024, block_size=64, max_blocks=16, mlp4_act4=act4))
+        seq = Sequence(rt)
+        lg = seq.prefill(prompt, chunk=64)
+        coss = [_close(lg[0], ref_logits[0])[0]]
+        for i, t in enumerate(toks[:-1]):
+            lg = seq.verify([t])
+            seq.commit(1)
+            coss.append(_close(lg[0], ref_logits[i + 1])[0])
+        # act4: the prompt's MLP activations are quantised, and with them the state that decoding starts from
+        assert min(coss) > (0.95 if act4 else 0.999), (act4, coss)
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("rows", [1, 8, 40])
+def test_shared_expert_mlp4(tiny_ckpt, tiny_cfg, fmt, rows):
+    """A MoE layer whose shared expert is in 4 bits: the routed sum of an fp8 run plus the block in 64 bits, on the side
+    stream (decode windows) and after the routed experts."""
+    from glm53.models import weights as W
+    from glm53.models.runtime import Runtime, RuntimeConfig
+    from glm53.ops import fp4
+    rc = RuntimeConfig(max_rows=48, kv_slots=256, max_blocks=4)
+    w4 = W.prepare(W.DictSource(tiny_ckpt), tiny_cfg, device=DEV, mlp4=fmt)
+    w8 = W.prepare(W.DictSource(tiny_ckpt), tiny_cfg, device=DEV)
+    lw4, lw8 = w4.layers[1], w8.layers[1]
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x = torch.randn(rows, tiny_cfg.hidden, generator=g, device=DEV).to(torch.bfloat16)
+    p = "model.layers.1.mlp.shared_experts."
+    gate, up, down = (fp4.dequantize4(fp4.quantize4(tiny_ckpt[p + n + "_proj.weight"].to(DEV).to(torch.bfloat16), fmt),
+                                      torch.float32).double() for n in ("gate", "up", "down"))
+    lim = tiny_cfg.limit
+    gv, uv = (x.double() @ gate.t()).clamp(max=lim), (x.double() @ up.t()).clamp(-lim, lim)
+    h = (gv * torch.sigmoid(gv) * uv).to(torch.bfloat16).double()
+    ref = h @ down.t()
+    outs = {}
+    for name, w, lw in (("4", w4, lw4), ("8", w8, lw8)):
+        for overlap in (True, False):
+            rt = Runtime(w, rc)
+            rt.overlap = rt.overlap and overlap
+            rt._keep_window, rt._sp, rt._fused = True, None, False
+            rt.normed[:rows] = x
+            rt._moe(lw, rows)
+            torch.cuda.synchronize()
+            outs[name, overlap] = rt.branch[:rows].double()
+    m = w8.layers[1].moe.shared
+    g8 = x.double() @ (m.gu.w.view(torch.float8_e4m3fn).double() * m.gu.s.double()[:, None]).t()
+    n = m.width
+    rb = lambda t: t.to(torch.bfloat16).double()                                  # noqa: E731
+    gv, uv = rb(g8[:, :n]).clamp(max=lim), rb(g8[:, n:]).clamp(-lim, lim)
+    ref8 = rb(gv * torch.sigmoid(gv) * uv) @ (m.down.w.view(torch.float8_e4m3fn).double() * m.down.s.double()[:, None]).t()
+    routed = outs["8", False] - ref8
+    # h (and, in the fp8 run, gate and up) may round to bf16 on either side: half a step each, 2^-8 of the magnitudes
+    tol = 2.0 ** -8 * (h.abs() @ down.abs().t()) + 3 * 2.0 ** -8 * (rb(gv * torch.sigmoid(gv) * uv).abs() @ (
+        m.down.w.view(torch.float8_e4m3fn).double().abs() * m.down.s.double()[:, None]).t()) + 1e-5 * outs["8", False].abs()
+    for overlap in (True, False):
+        assert ((outs["4", overlap] - (routed + ref)).abs() <= tol).all()
+
+
+def test_engine_with_mlp4_graphs():
+    """The engine (CUDA graphs, speculation, side stream) on 4-bit MLPs: the tokens of a run without graphs."""
+    from glm53.api.offline import LLM, LLMOptions
+    from glm53.engine.llm import SamplingParams
+    outs = []
+    for graphs in (True, False):
+        llm = LLM(LLMOptions(model="tiny", max_seqs=2, max_model_len=512, prefill_chunk=128, mlp4="nvfp4", mlp4_act4=True,
+                             cuda_graphs=graphs, k_fixed=4))
+        outs.append([o["token_ids"] for o in llm.generate([[1, 2, 3] * 50, [9, 8, 7] * 20],
+                                                          SamplingParams(max_tokens=24))])
+    assert outs[0] == outs[1]
