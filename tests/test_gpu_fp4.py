@@ -172,6 +172,17 @@ def test_linear_few_rows(fmt, n, k, m):
     assert torch.equal(fp4.linear4(x, w4, torch.empty_like(y), K.GEMV_F32, act4=True), y)     # 16 rows: exact
 
 
+@pytest.mark.parametrize("k", [16, 48, 80, 272])
+def test_linear_nv_takes_any_multiple_of_16(k):
+    w = weight(70, k, k)
+    w4, wq = fp4.quantize4(w, "nvfp4"), quant(w, "nvfp4")
+    for m, act4 in ((1, False), (20, False), (300, False), (20, True), (300, True)):
+        x = acts(m, k, m)
+        a = quant(x, "nvfp4") if act4 else x.double()
+        y = fp4.linear4(x, w4, torch.empty(m, 70, dtype=F32, device="cuda"), K.GEMV_F32, act4=act4)
+        assert ((y.double() - a @ wq.t()).abs() <= sums_tol(a, wq) + act_tol(a, wq, "nvfp4")).all(), (m, act4)
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_linear_few_rows_magnitudes_and_views(fmt):
     n, k = 200, 576
@@ -425,6 +436,43 @@ def test_weights_written_just_before_their_product():
         y = fp4.linear4(x, w4, torch.empty(4, 2048, dtype=F32, device="cuda"), K.GEMV_F32)
         torch.cuda.synchronize()
         assert torch.equal(y, fp4.linear4(x, w4, torch.empty_like(y), K.GEMV_F32))
+
+
+def test_first_calls_inside_a_capture():
+    """In a fresh process, each product's first launch may be a captured one."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, sys
+sys.path.insert(0, sys.argv[1])
+from glm53.ops import fp4, kernels as K
+w = fp4.quantize4(torch.randn(256, 512, device='cuda').to(torch.bfloat16))
+m = fp4.pack_mlp4(*(torch.randn(64, 512, device='cuda').to(torch.bfloat16) for _ in range(2)),
+                  torch.randn(96, 64, device='cuda').to(torch.bfloat16))
+xs = [torch.randn(r, 512, device='cuda').to(torch.bfloat16) for r in (1, 12, 30, 300)]
+def calls():
+    out = []
+    for x in xs:
+        for act4 in (False, True):
+            y = torch.empty(x.shape[0], 256, device='cuda', dtype=torch.float32)
+            z = torch.empty(x.shape[0], 96, device='cuda', dtype=torch.float32)
+            out += [fp4.linear4(x, w, y, K.GEMV_F32, act4=act4), fp4.mlp4(x, m, z, 10.0, act4=act4),
+                    fp4.dequantize4(fp4.quantize4(x, 'mxfp4'))]
+    return out
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = calls()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+fp4.check_errors()
+print('captured', len(got))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code, root], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "captured 24" in r.stdout, r.stderr[-2000:]
 
 
 def test_empty_batch():
