@@ -38,15 +38,14 @@ __device__ __forceinline__ int chunk_off(int r, int c) { return r * 128 + ((c ^ 
 // byte of block column s of row r inside a scale tile
 __device__ __forceinline__ int scale_off(int r, int s) { return (s >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (s & 3); }
 
-// 8 codes (one 32-bit word) -> four f16x2, exact; o[i] holds codes 2i (low half) and 2i + 1.  Through CUDA's function,
-// a byte at a time: an inline unpack of the word into four .b8 registers came out of the assembler (12.9) with bytes
-// exchanged or lost, depending on what stood before it.
+// 8 codes (one 32-bit word) -> four f16x2, exact; o[i] holds codes 2i (low half) and 2i + 1.  Each byte goes into its .b8
+// register through an explicit conversion: 62 values a clock and SM, 25 through CUDA's function of one byte.  (Unpacking
+// the word into four .b8 registers at once came out of the assembler, 12.9, with bytes exchanged or lost, depending on what
+// stood before it.)
 __device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&o)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((w >> (8 * i)) & 0xffu), __NV_E2M1);
-    o[i] = (uint32_t)h.x | ((uint32_t)h.y << 16);
-  }
+  for (int i = 0; i < 4; ++i)
+    asm("{\n .reg .b8 a;\n cvt.u8.u32 a, %1;\n cvt.rn.f16x2.e2m1x2 %0, a;\n}\n" : "=r"(o[i]) : "r"(w >> (8 * i)));
 }
 // 8 values -> 8 codes (nearest, ties to even, saturating at 6)
 __device__ __forceinline__ uint32_t f32x8_to_e2m1(const float (&v)[8]) {

@@ -19,8 +19,9 @@ using OptT = c10::optional<Tensor>;
 
 constexpr int64_t kTileRows = 128, kTileK = 256, kTileBytes = 16384;
 constexpr int64_t kFourRows = 16;      // rows above which act4 quantises the activations
-constexpr int64_t kGemmRows = 256;     // rows above which exact activations go through the bf16 tcgen05 GEMM (4096 x 4096: 200
-                                       // rows 28.5 us, 34.5 there; 300 rows 37.6, 34.6)
+constexpr int64_t kFewRows = 96;       // rows up to which exact activations are expanded into 4-bit terms (24576 x 4096: 96 rows
+                                       // 48 us, 57 widened; 112 rows 67, 57.  4096 x 4096: 96 rows 16.3, 16.7; 112 rows 18.0,
+                                       // 16.9.  A 4096 x 12288 weight would gain from 64 rows on, 4096 x 2048 from 160)
 constexpr int64_t kFour = 128;         // rows up to which 4-bit activations go through the small-M kernel (24576 x 4096: 100 rows
                                        // 28.8 us, 36.3 on the GEMM; 200 rows 42.6, 35.5)
 
@@ -124,7 +125,7 @@ Matrix4 quantize(const Tensor& x, bool nv) {
   return m;
 }
 
-void dequant(const Matrix4& m, const Tensor& y, int64_t il) {
+void dequant(const Matrix4& m, const Tensor& y) {
   Fp4DequantArgs a{};
   a.codes = m.codes;
   a.scales = m.scales;
@@ -133,7 +134,6 @@ void dequant(const Matrix4& m, const Tensor& y, int64_t il) {
   a.K = m.k;
   a.nv = m.nv;
   a.out = y.scalar_type() == at::kBFloat16 ? 0 : y.scalar_type() == at::kHalf ? 1 : 2;
-  a.il = il;
   a.y = y.data_ptr();
   a.ldy = y.stride(0);
   a.vec = aligned16(a.y) && (a.ldy * y.element_size()) % 16 == 0;
@@ -151,7 +151,7 @@ Tensor dequantize(const Matrix4& m, const OptT& out, at::ScalarType dtype) {
   TORCH_CHECK(y.dim() == 2 && y.size(0) == m.rows && y.size(1) == m.k && y.stride(1) == 1 &&
                   (m.rows == 1 || y.stride(0) >= m.k),
               "dequantize4: the output must be [", num(m.rows), ", ", num(m.k), "], rows contiguous and apart");
-  dequant(m, y, 0);
+  dequant(m, y);
   return y;
 }
 
@@ -229,29 +229,27 @@ void skinny4(const Matrix4& x, float factor, const Matrix4& w, const Tensor& y, 
   ok(g53_fp4_skinny(a, stream()), "fp4_skinny");
 }
 
-// exact activations, many rows: the weights widened to bf16 (every 4-bit value times its scales is a bf16 value), then
-// the bf16 tcgen05 GEMM
-void gemm_exact(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t n, int64_t il, int64_t mode, double limit) {
-  Tensor xx = aligned16(x.data_ptr()) && x.stride(0) % 8 == 0 ? x : x.contiguous().clone();
-  const Tensor wb = at::empty({n, w.k}, x.options());
-  dequant(w, wb, il);
-  GemmArgs p{};
-  p.a = xx.data_ptr();
-  p.lda = xx.stride(0);
-  p.b = wb.data_ptr();
-  p.ldb = wb.stride(0);
-  p.y = y.data_ptr();
-  p.ldy = y.stride(0);
-  p.M = (int)x.size(0);
-  p.N = (int)n;
-  p.K = (int)w.k;
-  p.mode = (int)mode;
-  p.limit = (float)limit;
-  // 128-column tiles where they still are one wave (500 x 4096 x 12288: 93 us, 107 with 256; where they are two, 300 rows
-  // of 24576 x 4096 stay at 121 and 800 of 4096 x 4096 would take 57 instead of 38)
-  if ((x.size(0) + 127) / 128 * ((n + 127) / 128) <= at::cuda::getCurrentDeviceProperties()->multiProcessorCount) p.bn = 128;
-  ok(g53_fp4_gemm_error_word(&p.err), "fp4 error word");
-  ok(g53_gemm_sm100(p, stream()), "gemm_sm100");
+// exact activations, more rows: the weights widened inside the product
+void exact(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t width, int64_t mode, double limit) {
+  // rows that the tensor map cannot describe (unaligned, or broadcast) are copied
+  const bool direct = aligned16(x.data_ptr()) && x.stride(0) % 8 == 0 && x.stride(0) >= w.k;
+  const Tensor xx = direct ? x : x.clone(at::MemoryFormat::Contiguous);
+  Fp4ExactArgs a{};
+  a.x = reinterpret_cast<const __nv_bfloat16*>(xx.data_ptr());
+  a.ldx = xx.stride(0);
+  a.codes = w.codes;
+  a.scales = w.scales;
+  a.row_scale = w.row_scale;
+  a.nv = w.nv;
+  a.y = y.data_ptr();
+  a.ldy = y.stride(0);
+  a.M = (int)x.size(0);
+  a.N = (int)w.rows;
+  a.K = (int)w.k;
+  a.width = (int)width;
+  a.mode = (int)mode;
+  a.limit = (float)limit;
+  ok(g53_fp4_exact(a, stream()), "fp4_exact");
 }
 
 Fp4GemmArgs gemm_args(const Matrix4& a, const Matrix4& w, int64_t mode) {
@@ -286,8 +284,8 @@ void linear(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t mode, bo
     p.y = y.data_ptr();
     p.ldy = y.stride(0);
     ok(g53_fp4_gemm(p, stream()), "fp4_gemm");
-  } else if (M > kGemmRows) {
-    gemm_exact(x, w, y, w.rows, 0, mode, 0.0);
+  } else if (M > kFewRows) {
+    exact(x, w, y, 0, mode, 0.0);
   } else {
     skinny(x, w, y, 0, mode, 0.0);
   }
@@ -339,9 +337,9 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
     return;
   }
   const Tensor h = at::empty({M, W}, x.options());
-  if (M > kGemmRows) {
-    gemm_exact(x, gu, h, 2 * W, W, GEMV_SWIGLU_F32, limit);
-    gemm_exact(h, down, y, down.rows, 0, mode, 0.0);
+  if (M > kFewRows) {
+    exact(x, gu, h, W, GEMV_SWIGLU, limit);
+    exact(h, down, y, 0, mode, 0.0);
     return;
   }
   skinny(x, gu, h, W, GEMV_SWIGLU, limit);
@@ -350,10 +348,11 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
 
 int64_t error(int64_t device) {
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
-  int a = 0, b = 0;
+  int a = 0, b = 0, c = 0;
   ok(g53_fp4_skinny_error(&a), "fp4_skinny_error");
   ok(g53_fp4_gemm_error(&b), "fp4_gemm_error");
-  return a ? a : b;
+  ok(g53_fp4_exact_error(&c), "fp4_exact_error");
+  return a ? a : b ? b : c;
 }
 
 }  // namespace

@@ -1,0 +1,510 @@
+// Product with 4-bit weights and bf16 activations for more rows than the expansion serves: Y[M, N] = X[M, K] @ W4[N, K]^T,
+// W4A16.  Every 4-bit value times its block scale is a bf16 value, so the weights are widened to bf16 on the way into the
+// tensor core and nothing is rounded; the nvfp4 row scale is applied to the fp32 sums.
+//
+// A pair of CTAs (tcgen05.mma kind::f16, cta_group::2) takes 256 rows of W, 128 each, x up to 512 rows of X (the mma's
+// columns, one or two mma wide), and a slice of K; a cluster of CL pairs shares a tile.  Of X each CTA fetches one half: the
+// re-reading of X by every block of W is what the L2 has to carry (a CTA on its own with all of it: 300 rows x 24576 x 4096
+// 111 us, 73 in pairs).  Warp roles:
+//   warp 0     X tiles (64 columns, TMA with 128-byte swizzle) into a ring
+//   warp 1     allocates TMEM; one thread of the pair's first CTA issues four mma (K = 16) per stage and column half; that of
+//              the second passes on that its stage is ready
+//   warp 2     4-bit tiles (128 x 256: one contiguous cp.async.bulk of codes, one of scales) into a second ring
+//   warps 3-18 widen, in two sets of 8 that take the ring's stages in turn: a thread half a row of 64 columns (one 16-byte
+//              chunk), written as the swizzled operand; then the epilogue
+// Bound: a stage takes the tensor core 2 clocks per row of X (512 rows: 1007 measured) and the widening warps about 600 (64
+// rows; 850 with one set, no better with three), so from 300 rows on the mma sets the pace and below the widening.  Writing
+// the widened weights to memory for a bf16 product would cost 4 1/2 bytes of traffic per weight instead of 9/16: 300 rows
+// x 24576 x 4096 121 us (73 here), 300 x 4096 x 12288 101 (44), 2000 x 24576 x 4096 354 (306), 8192 x 12288 x 4096 621 (618).
+//
+// The slices of a cluster are written as fp32 to each CTA's shared memory and added in rank order by the rank that owns the
+// rows, so the result does not depend on timing.  Waits are bounded; one that runs out sets the error word, the roles stop
+// issuing, wait for what they have in flight, every barrier is still reached and the TMEM is freed.
+#include <cuda.h>
+#include <algorithm>
+#include <atomic>
+#include "fp4.cuh"
+#include "fp4_tc.cuh"
+#include "launchers.h"
+
+namespace g53 {
+namespace fp4 {
+
+__device__ int g_exact_err = 0;
+
+constexpr int kSets = 2;                              // sets of 8 warps that widen, stage by stage in turn
+constexpr int kWiden = 8 * kSets;
+constexpr int kRoles = 3;                             // warps that feed and issue
+constexpr int kExThreads = (kRoles + kWiden) * 32;
+constexpr int kWStages = 3;                           // 4-bit tiles in flight
+constexpr int kABytes = 128 * 128;                    // a stage's bf16 weights: 128 rows x 64
+
+constexpr int kPass = 256;                            // rows of X whose sums lie in shared memory at a time
+constexpr int kMaxCols = 512;                         // rows of X of a pair: all of TMEM
+
+struct ExPlan {
+  int KT, per, CL, ncol, mmas, groups, stages, stage_bytes;
+};
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t dup_bf16(float v) {
+  const __nv_bfloat162 b = __float2bfloat162_rn(v);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+// 8 codes -> 8 bf16, times s.  The bits of a code (sign, two of exponent, one of mantissa) at 15 and 8..6 of a bf16 are the
+// value x 2^-126, its subnormal 1/2 included: a byte permutation lays two codes into the halves of a word (its sign mode
+// gives the zero bytes), one multiplication copies them to both places, a mask keeps the bits wanted.  The scale brings the
+// exponent: for nvfp4 s = scale x 2^118, so the result is 2^-8 of the weight (the epilogue makes it up); an E8M0 scale may be
+// as large as a bf16, so mxfp4 multiplies twice.  Every product is exact.
+template <bool NV>
+__device__ __forceinline__ uint4 widen8(uint32_t w, uint32_t s) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;            // codes 0, 2, 4, 6 and 1, 3, 5, 7
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t t;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(t) : "r"(lo), "r"(hi), "r"(0xc480 + 0x1111 * i));
+    v[i] = (t * 0x1040u) & 0x81c081c0u;
+    if constexpr (!NV) v[i] = mul_bf16x2(v[i], 0x7e807e80u);
+    v[i] = mul_bf16x2(v[i], s);
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void tma_2d(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(tc::saddr(dst)), "l"(map), "r"(x), "r"(y), "r"(tc::saddr(bar)) : "memory");
+}
+// a wait that mostly finds its barrier done: every lane looks once, and one lane polls after that
+__device__ __forceinline__ bool look(uint64_t* b, uint32_t ph, volatile int* fail, int code) {
+  return __all_sync(0xffffffffu, tc::bar_try(b, ph)) || tc::warp_wait(b, ph, fail, &g_exact_err, code);
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void ex_store(const Fp4ExactArgs& p, int64_t tok, int n, float v) {
+  const int64_t off = tok * p.ldy + n;
+  if (p.mode == GEMV_BF16) {
+    reinterpret_cast<__nv_bfloat16*>(p.y)[off] = f2bf(v);
+  } else {
+    float* y = reinterpret_cast<float*>(p.y) + off;
+    *y = p.mode == GEMV_F32_ACC ? *y + v : v;
+  }
+}
+
+template <bool NV>
+__global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_constant__ CUtensorMap xmap, Fp4ExactArgs p,
+                                                                  ExPlan pl) {
+  constexpr int kSB = Fmt<NV>::kScaleBytes, kWBytes = kTileBytes + kSB;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t wfull[kWStages], wempty[kWStages], full[8], empty[8], tfull, drain;
+  __shared__ uint32_t tmem_s;
+  __shared__ int fail_s;
+  volatile int* fail = &fail_s;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* wring = ring + pl.stages * pl.stage_bytes;
+  float* part = reinterpret_cast<float*>(ring);       // sums [row of X][128], over the ring when it is done
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int CL = pl.CL, size = 2 * CL, crank = (int)blockIdx.x % size;
+  const int side = crank & 1, rank = crank >> 1;       // which 128 rows of the pair, which slice of K
+  const int unit = (int)blockIdx.x / size;
+  const int pb = unit / pl.groups, x0 = (unit - pb * pl.groups) * pl.ncol;
+  const int nb = 2 * pb + side;
+  const int nb_ld = min(nb, (p.N + 127) / 128 - 1);    // an odd last block: its partner widens it once more, and stores nothing
+  const int M = min(p.M - x0, pl.ncol);
+  const int t_lo = rank * pl.per, t_hi = min(pl.KT, t_lo + pl.per);
+  const int n_st = min(t_hi * 4, (p.K + 63) / 64) - t_lo * 4;          // stages of 64 columns
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kWStages; ++s) {
+      tc::bar_init(&wfull[s], 1);
+      tc::bar_init(&wempty[s], kWiden);
+    }
+    for (int s = 0; s < pl.stages; ++s) {
+      // its own copies and widening warps; rank 0 of a pair also word from rank 1 that its are done
+      tc::bar_init(&full[s], 1 + 8 + (side == 0 ? 1 : 0));
+      tc::bar_init(&empty[s], 1);
+    }
+    tc::bar_init(&tfull, 1);
+    tc::bar_init(&drain, 1);
+    fail_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc_pair(&tmem_s, 512);
+  tc::fence_before();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  tc::fence_after();
+  const uint32_t tmem = tmem_s;
+  pdl_trigger();
+  bool live = true;                                    // a widening warp that has not given up
+
+  if (warp == 0) {
+    if (elect_one()) {
+      pdl_wait();
+      const int cols = pl.ncol / pl.mmas, mine = cols / 2;             // rows of X of one mma, and those that this CTA holds
+      int st = 0, s = 0, ph = 1;
+      for (; st < n_st; ++st) {
+        if (st >= pl.stages && !tc::bar_wait(&empty[s], ph, fail, &g_exact_err, 1)) break;
+        uint8_t* dst = ring + s * pl.stage_bytes + kABytes;
+        bulk_expect(&full[s], (uint32_t)pl.ncol * 64);
+        for (int h = 0; h < pl.mmas; ++h)
+          tma_2d(&xmap, &full[s], dst + h * mine * 128, (t_lo * 4 + st) * 64, x0 + h * cols + side * mine);
+        if (++s == pl.stages) { s = 0; ph ^= 1; }
+      }
+      if (*fail) {
+        // the copies in flight land before the CTA ends: they are counted on barriers that also wait for the widening warps,
+        // which arrive in a stopped CTA, too
+        int none = 0;
+        for (int j = max(0, st - pl.stages); j < st; ++j) tc::bar_wait(&full[j % pl.stages], (j / pl.stages) & 1, &none, nullptr, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    if (elect_one()) {
+      int wt = 0;
+      for (; wt < t_hi - t_lo; ++wt) {
+        const int w = wt % kWStages;
+        if (wt >= kWStages && !tc::bar_wait(&wempty[w], ((wt / kWStages) - 1) & 1, fail, &g_exact_err, 2)) break;
+        const int64_t tile = (int64_t)nb_ld * pl.KT + t_lo + wt;
+        if (wt == 0) pdl_wait();
+        bulk_expect(&wfull[w], kWBytes);
+        bulk_load(wring + w * kWBytes, p.codes + tile * kTileBytes, kTileBytes, &wfull[w]);
+        bulk_load(wring + w * kWBytes + kTileBytes, p.scales + tile * kSB, kSB, &wfull[w]);
+      }
+      if (*fail) {
+        int none = 0;
+        for (int j = max(0, wt - kWStages); j < wt; ++j) tc::bar_wait(&wfull[j % kWStages], (j / kWStages) & 1, &none, nullptr, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      bool ok = true;
+      int s = 0, ph = 0;
+      if (side == 1) {
+        for (int st = 0; st < n_st; ++st) {
+          if (!tc::bar_wait(&full[s], ph, fail, &g_exact_err, 3)) break;
+          signal_at(&full[s], crank & ~1);
+          if (++s == pl.stages) { s = 0; ph ^= 1; }
+        }
+      } else {
+        const int cols = pl.ncol / pl.mmas;
+        const uint32_t id = tc::idesc(1, cols, 256);
+        const uint16_t both = (uint16_t)(3u << crank);
+        uint32_t acc = 0;
+        for (int st = 0; st < n_st; ++st) {
+          if (!tc::bar_wait(&full[s], ph, fail, &g_exact_err, 7)) { ok = false; break; }
+          tc::fence_after();
+          const uint32_t sa = tc::saddr(ring + s * pl.stage_bytes);
+          const uint64_t a = tc::desc_sw128(sa), b = tc::desc_sw128(sa + kABytes), b2 = tc::desc_sw128(sa + kABytes + cols * 64);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            mma_pair(tmem, a + 2 * k, b + 2 * k, id, acc);             // 32 bytes on in the descriptors' units of 16
+            if (pl.mmas == 2) mma_pair(tmem + cols, a + 2 * k, b2 + 2 * k, id, acc);
+            acc = 1;
+          }
+          commit_pair(&empty[s], both);
+          if (++s == pl.stages) { s = 0; ph ^= 1; }
+        }
+        if (ok) {
+          commit_pair(&tfull, both);
+        } else {
+          int none = 0;
+          commit_pair(&drain, both);
+          tc::bar_wait(&drain, 0, &none, nullptr, 0);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int ww = warp - kRoles, set = ww >> 3;
+    const int row = (ww & 7) * 16 + (lane >> 1), half = lane & 1;            // 32 of the stage's 64 columns of a row
+    const int flip = (row & 7) << 4;                    // the swizzle of this row
+    const uint8_t* codes = wring + row * 128;
+    const uint8_t* scales = wring + kTileBytes + scale_off(row, NV ? 2 * half : half);
+    uint8_t* out = ring + row * 128;
+    int s = set, ph = 1, w = 0, wph = 0, j = set;       // ring slot and its phase, 4-bit tile and its phase, stage of the tile
+    if (n_st > set) live = look(&wfull[0], 0, fail, 4);
+    for (int st = set; st < n_st; st += kSets) {
+      if (live && st >= pl.stages) live = look(&empty[s], ph, fail, 5);
+      if (live) {
+        const uint4 q = *reinterpret_cast<const uint4*>(codes + w * kWBytes + ((j * 32 + half * 16) ^ flip));
+        // the scales of 64 columns: 4 bytes of atom j (nvfp4), 2 bytes of atom j / 2
+        const uint8_t* sp = scales + w * kWBytes + (NV ? j * 512 : (j >> 1) * 512 + (j & 1) * 2);
+        uint32_t s0, s1;
+        if constexpr (NV) {
+          const uint32_t h = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(sp));
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          s0 = dup_bf16(f.x * 0x1p118f);
+          s1 = dup_bf16(f.y * 0x1p118f);
+        } else {
+          s0 = s1 = dup_bf16(e8m0_to_f32(*sp));
+        }
+        uint8_t* dst = out + s * pl.stage_bytes;
+        *reinterpret_cast<uint4*>(dst + ((half * 64) ^ flip)) = widen8<NV>(q.x, s0);
+        *reinterpret_cast<uint4*>(dst + ((half * 64 + 16) ^ flip)) = widen8<NV>(q.y, s0);
+        *reinterpret_cast<uint4*>(dst + ((half * 64 + 32) ^ flip)) = widen8<NV>(q.z, s1);
+        *reinterpret_cast<uint4*>(dst + ((half * 64 + 48) ^ flip)) = widen8<NV>(q.w, s1);
+        tc::fence_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) tc::bar_arrive(&full[s]);
+      s += kSets;
+      if (s >= pl.stages) { s -= pl.stages; ph ^= 1; }
+      j += kSets;
+      if (j > 3) {                                      // its last stage of the tile
+        if (lane == 0) tc::bar_arrive(&wempty[w]);
+        j -= 4;
+        if (++w == kWStages) { w = 0; wph ^= 1; }
+        if (live && st + kSets < n_st) live = look(&wfull[w], wph, fail, 4);
+      }
+    }
+    pdl_wait();
+    if (live) live = tc::warp_wait(&tfull, 0, fail, &g_exact_err, 6);
+    tc::fence_after();
+  }
+  // ---- sums: a thread holds one row of W; those of the cluster meet in shared memory
+  const bool swi = p.mode == GEMV_SWIGLU, meet = CL > 1 || swi;
+  for (int cb = 0; cb < M; cb += kPass) {
+    const int ce = min(M, cb + kPass);
+    if (warp >= kRoles) {
+      const int ww = warp - kRoles, r = (warp & 3) * 32 + lane, n = nb * 128 + r;
+      const float rs = NV && n < p.N ? __ldcg(p.row_scale + n) : 1.f;
+      for (int c0 = cb + (ww >> 2) * 32; c0 < ce; c0 += kWiden / 4 * 32) {
+        float v[32];
+        if (live) tc::tmem_ld32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (c0 + i >= ce) break;
+          if (NV) v[i] *= 256.f;
+          if (!meet) {
+            if (n < p.N) ex_store(p, x0 + c0 + i, n, v[i] * rs);
+          } else {
+            part[(c0 + i - cb) * 128 + r] = v[i] * rs;
+          }
+        }
+      }
+    }
+    if (!meet) continue;
+    // every CTA of the cluster has its sums in shared memory
+    if (CL > 1) {
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+    if (warp >= kRoles) {
+      const int et = threadIdx.x - kRoles * 32, pairs = (64 + CL - 1) / CL;
+      const int j_lo = rank * pairs, cnt = min(64, j_lo + pairs) - j_lo;
+      const uint32_t base = tc::saddr(part);
+      for (int e = et; e < (ce - cb) * pairs; e += kWiden * 32) {
+        const int c = e / pairs, tok = x0 + cb + c, r = j_lo + e - c * pairs;
+        if (r >= j_lo + cnt) continue;
+        float v = 0.f, u = 0.f;
+        for (int k = 0; k < CL; ++k) {
+          uint32_t a = base + (c * 128 + r) * 4;
+          asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(a) : "r"(CL > 1 ? 2 * k + side : crank));
+          v += ld_cluster(a);
+          u += ld_cluster(a + 64 * 4);
+        }
+        const int n = nb * 128 + r;
+        if (swi) {
+          const int col = nb * 64 + r;
+          if (col >= p.width) continue;
+          // written so that a NaN stays one
+          v = v > p.limit ? p.limit : v;
+          u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
+          reinterpret_cast<__nv_bfloat16*>(p.y)[(int64_t)tok * p.ldy + col] = f2bf(siluf_(v) * u);
+        } else {
+          if (n < p.N) ex_store(p, tok, n, v);
+          if (n + 64 < p.N) ex_store(p, tok, n + 64, u);
+        }
+      }
+    }
+    // no CTA overwrites its sums while another reads them
+    if (ce < M) {
+      __syncwarp();
+      if (CL > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        cluster_wait();
+      } else {
+        __syncthreads();
+      }
+    }
+  }
+  // nor leaves while its memory or its partner's part of the accumulator is in use
+  tc::fence_before();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  if (warp == 1) {
+    tc::fence_after();
+    tmem_free_pair(tmem, 512);
+  }
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+  static std::atomic<EncodeTiled> known{nullptr};
+  EncodeTiled fn = known.load(std::memory_order_relaxed);
+  if (!fn) {
+    void* q = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) == cudaSuccess &&
+        r == cudaDriverEntryPointSuccess)
+      known.store(fn = reinterpret_cast<EncodeTiled>(q), std::memory_order_relaxed);
+  }
+  return fn;
+}
+
+constexpr int kExBudget = 225 * 1024, kMaxSplit = 3, kMaxDev = 64;
+
+// Stands in for the product in the question below: the runtime answers wrongly for a kernel that uses TMEM
+__global__ void __launch_bounds__(kExThreads, 1) ex_shape_kernel() {}
+
+// clusters of 2 * cl CTAs that run at once on the current device, one CTA per SM; asked once per device
+static cudaError_t ex_active(int dev, int cl, int* out) {
+  static std::atomic<int> known[kMaxDev][kMaxSplit + 1];
+  if (dev < kMaxDev && (*out = known[dev][cl].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(ex_shape_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kExBudget);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * cl);
+  cfg.blockDim = dim3(kExThreads);
+  cfg.dynamicSmemBytes = kExBudget;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2 * cl;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(out, ex_shape_kernel, &cfg);
+  if (e != cudaSuccess) return e;
+  *out = std::max(*out, 1);
+  if (dev < kMaxDev) known[dev][cl].store(*out, std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
+// Shape: groups of rows of X and K split with the least time, in clocks.  A stage of 64 columns takes the widening (500) or
+// the mma (2 per row of X, and 60); a tile 7000 and 8 per row beside that, the exchange of a cluster 4000 and 12 per row.
+// Fitted to a sweep of both over 16 row counts from 64 to 8192 and seven weight sizes: the shape chosen is 2% from the best
+// of the sweep on average, 28% at worst.  An eighth of the clusters' room stays free, as one that has to wait doubles the time.
+template <bool NV>
+static cudaError_t launch_exact(const Fp4ExactArgs& p, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  auto kern = fp4_exact_kernel<NV>;
+  static std::atomic<bool> ready[64];                 // the shared memory limit, raised once per device
+  if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kExBudget);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  }
+  ExPlan b{};
+  b.KT = tiles_k(p.K);
+  const int64_t pairs = ((int64_t)p.N + 255) / 256;
+  double best = 0;
+  const int fewest = (p.M + kMaxCols - 1) / kMaxCols;
+  for (int want = fewest; want <= fewest + 3; ++want) {
+    int ncol = ((p.M + want - 1) / want + 15) / 16 * 16;
+    const int mmas = ncol > 256 ? 2 : 1;              // an mma has 256 columns at most; two are equally wide
+    ncol = (ncol + 16 * mmas - 1) / (16 * mmas) * (16 * mmas);
+    const int groups = (p.M + ncol - 1) / ncol;
+    for (int cl = 1; cl <= kMaxSplit && cl <= b.KT; ++cl) {
+      const int per = (b.KT + cl - 1) / cl;
+      if ((b.KT + per - 1) / per != cl) continue;      // a CTA would have no tile
+      int active = 0;
+      e = ex_active(dev, cl, &active);
+      if (e != cudaSuccess) return e;
+      if (cl > 1) active -= active / 8;
+      const int64_t units = pairs * groups;
+      const double t = (double)((units + active - 1) / active) *
+                       (per * 4.0 * std::max(500, 2 * ncol + 60) + 7000 + 8 * ncol + (cl > 1 ? 4000 + 12 * ncol : 0));
+      if (b.CL == 0 || t < best) {
+        best = t;
+        b.CL = cl;
+        b.per = per;
+        b.ncol = ncol;
+        b.mmas = mmas;
+        b.groups = groups;
+      }
+    }
+  }
+  if (b.CL == 0) return cudaErrorNotSupported;
+  const int64_t units = pairs * b.groups;
+  if (units * 2 * kMaxSplit >= (int64_t)1 << 31) return cudaErrorInvalidConfiguration;
+  constexpr int kWBytes = kTileBytes + Fmt<NV>::kScaleBytes;
+  b.stage_bytes = kABytes + b.ncol * 64;
+  b.stages = std::min(8, (kExBudget - 1024 - kWStages * kWBytes) / b.stage_bytes);
+  // the sums lie over both rings
+  const int smem = std::max(b.stages * b.stage_bytes + kWStages * kWBytes, std::min(b.ncol, kPass) * 512) + 1024;
+
+  EncodeTiled fn = encode_tiled();
+  if (!fn) return cudaErrorNotSupported;
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.ldx * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)(b.ncol / b.mmas / 2)}, es[2] = {1, 1};
+  if (fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<__nv_bfloat16*>(p.x), dims, strides, box, es,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * b.CL * 2));
+  cfg.blockDim = dim3(kExThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int na = 0;
+  at[na].id = cudaLaunchAttributeClusterDimension;
+  at[na].val.clusterDim.x = 2 * b.CL;
+  at[na].val.clusterDim.y = 1;
+  at[na].val.clusterDim.z = 1;
+  ++na;
+  if (g53_pdl_on()) {
+    at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = na;
+  return cudaLaunchKernelEx(&cfg, kern, map, p, b);
+}
+
+}  // namespace fp4
+}  // namespace g53
+
+using namespace g53;
+
+cudaError_t g53_fp4_exact(const Fp4ExactArgs& p, cudaStream_t st) {
+  if (p.M < 1 || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32) || (reinterpret_cast<uintptr_t>(p.x) & 15) || p.ldx % 8 ||
+      p.ldx < p.K)
+    return cudaErrorInvalidValue;
+  return p.nv ? fp4::launch_exact<true>(p, st) : fp4::launch_exact<false>(p, st);
+}
+
+cudaError_t g53_fp4_exact_error(int* code) {
+  const int z = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(code, fp4::g_exact_err, sizeof(int));
+  if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(fp4::g_exact_err, &z, sizeof(int));
+  return e;
+}

@@ -497,10 +497,6 @@ cudaError_t g53_fp4_gemm(const Fp4GemmArgs& p, cudaStream_t st) {
   return p.nv ? fp4::gemm_t<true>(q, dev, sms, st) : fp4::gemm_t<false>(q, dev, sms, st);
 }
 
-cudaError_t g53_fp4_gemm_error_word(int** word) {
-  return cudaGetSymbolAddress(reinterpret_cast<void**>(word), fp4::g_gemm_err);
-}
-
 cudaError_t g53_fp4_gemm_error(int* code) {
   const int z = 0;
   cudaError_t e = cudaMemcpyFromSymbol(code, fp4::g_gemm_err, sizeof(int));

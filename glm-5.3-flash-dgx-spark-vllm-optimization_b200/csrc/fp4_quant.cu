@@ -171,9 +171,6 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(Fp4QuantArgs p) {
 
 // Read-back: a thread turns 8 codes (one word) into 8 outputs; 32 consecutive threads cover one tile row (256 columns),
 // so code loads are 128 contiguous bytes per warp and 16-bit stores 512.  Exact in fp32; rounded once to 16 bits.
-// il (gate/up images, fp4 row order of pack): row 128 b + j (j < 64) is gate row 64 b + j, row 128 b + 64 + j up row
-// 64 b + j; the output rows are the (8 gate, 8 up) interleave of the 16-bit GEMM's SwiGLU epilogue, rows of gate index
-// >= il skipped.
 // CTA: 8 rows (a warp each) x 8 tiles.
 constexpr int kDqTiles = 8;
 template <bool NV, int OUT>                           // OUT 0 bf16, 1 f16, 2 fp32
@@ -185,12 +182,6 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(Fp4DequantArgs p) {
   pdl_wait();
   if (row >= p.R) return;
   const int rr = (int)(row % kTileRows);
-  int64_t orow = row;
-  if (p.il > 0) {
-    const int64_t j = (row / 128) * 64 + (row % 64);
-    if (j >= p.il) return;
-    orow = (j / 8) * 16 + (j % 8) + ((row % 128) >= 64 ? 8 : 0);
-  }
   const float rs = NV ? __ldcg(p.row_scale + row) : 1.f;
   const int kt1 = min(KT, ((int)blockIdx.y + 1) * kDqTiles);
 #pragma unroll 4
@@ -211,7 +202,7 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(Fp4DequantArgs p) {
       v[2 * i] = f.x * s;
       v[2 * i + 1] = f.y * s;
     }
-    const int64_t off = orow * p.ldy + k0;
+    const int64_t off = row * p.ldy + k0;
     if constexpr (OUT == 2) {
       float* y = reinterpret_cast<float*>(p.y) + off;
       if (p.vec) {

@@ -62,10 +62,11 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
 }
 
 // ---- a pair of CTAs that share the mma: rank 0 issues, completions arrive on the same barrier of both
-__device__ __forceinline__ void commit_pair(uint64_t* b) {
+// (`both`: the two CTAs of the cluster)
+__device__ __forceinline__ void commit_pair(uint64_t* b, uint16_t both = 3) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-      ::"r"(tc::saddr(b)), "h"((uint16_t)3) : "memory");
+      ::"r"(tc::saddr(b)), "h"(both) : "memory");
 }
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::saddr(dst)), "r"(cols));

@@ -162,7 +162,7 @@ __device__ __forceinline__ void store_chunk(const GemmArgs& p, void* ybase, cons
 #pragma unroll
     for (int i = 0; i < 32; ++i) sc[i] = (bscale && nb + i < p.N) ? bscale[nb + i] : 1.f;
   }
-  if (p.mode == GEMV_SWIGLU || p.mode == GEMV_SWIGLU_F32) {
+  if (p.mode == GEMV_SWIGLU) {
     // columns: two groups of (8 gate rows, 8 matching up rows) of the interleaved weight -> 16 outputs
     __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(ybase) + (int64_t)row * p.ldy + (nb >> 1);
     float o[16];
@@ -170,15 +170,10 @@ __device__ __forceinline__ void store_chunk(const GemmArgs& p, void* ybase, cons
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float gv = v[g * 16 + i] * rs * sc[g * 16 + i];
-        float uv = v[g * 16 + 8 + i] * rs * sc[g * 16 + 8 + i];
-        if (p.mode == GEMV_SWIGLU_F32) {
-          gv = gv > p.limit ? p.limit : gv;
-          uv = uv > p.limit ? p.limit : uv < -p.limit ? -p.limit : uv;
-        } else {
-          gv = fminf(round_bf16(gv), p.limit);
-          uv = fminf(fmaxf(round_bf16(uv), -p.limit), p.limit);
-        }
+        float gv = round_bf16(v[g * 16 + i] * rs * sc[g * 16 + i]);
+        float uv = round_bf16(v[g * 16 + 8 + i] * rs * sc[g * 16 + 8 + i]);
+        gv = fminf(gv, p.limit);
+        uv = fminf(fmaxf(uv, -p.limit), p.limit);
         o[g * 8 + i] = siluf_(gv) * uv;
       }
     if (full) {
@@ -596,7 +591,7 @@ cudaError_t g53_gemm_sm100(const GemmArgs& p, cudaStream_t st) {
     return cudaErrorInvalidValue;
   if (p.batch > 1 && (((p.bsa * esz) & 15) || ((p.bsb * esz) & 15) || p.a_scale)) return cudaErrorInvalidValue;
   if (p.fp8) return p.N >= 256 ? launch<256, true, 4>(p, st) : launch<128, true, 6>(p, st);
-  return p.N >= 256 && p.bn != 128 ? launch<256, false, 4>(p, st) : launch<128, false, 6>(p, st);
+  return p.N >= 256 ? launch<256, false, 4>(p, st) : launch<128, false, 6>(p, st);
 }
 
 cudaError_t g53_quant_rows_e4m3(const __nv_bfloat16* x, int64_t ldx, int R, int K, uint8_t* q, float* scale,

@@ -7,9 +7,7 @@
 #include <stdint.h>
 
 // ---------------------------------------------------------------- small-M GEMM (gemv.cu)
-// GEMV_SWIGLU rounds gate and up to bf16 before the activation; GEMV_SWIGLU_F32 (gemm_sm100.cu) keeps them in fp32 and
-// lets a NaN through the clamps
-enum GemvMode { GEMV_BF16 = 0, GEMV_F32 = 1, GEMV_F32_ACC = 2, GEMV_SWIGLU = 3, GEMV_SWIGLU_F32 = 4 };
+enum GemvMode { GEMV_BF16 = 0, GEMV_F32 = 1, GEMV_F32_ACC = 2, GEMV_SWIGLU = 3 };
 
 struct GemvArgs {
   const __nv_bfloat16* x; int64_t ldx; int64_t bsx;   // activations [batch][M][K] (row stride ldx)
@@ -68,7 +66,6 @@ struct GemmArgs {
   float limit;
   int* err;                            // device error word (bounded waits that ran out)
   int vec;                             // set by the launcher: 16-byte epilogue stores allowed
-  int bn;                              // bf16: 128 = tiles of 128 columns even for N >= 256 (0: by N)
   // batched GEMM (e.g. per attention head): batch strides in elements of A, B, Y and of b_scale
   int batch;                           // 0 or 1: a single GEMM
   int64_t bsa, bsb, bsy, bss;
@@ -409,7 +406,6 @@ struct Fp4DequantArgs {
   int64_t R, K;
   int nv, out;                         // out: 0 bf16, 1 f16, 2 fp32
   int vec;                             // 16-byte aligned output rows
-  int64_t il;                          // > 0: gate/up image of this width, rows written in the (8 gate, 8 up) interleave
   void* y; int64_t ldy;
 };
 cudaError_t g53_fp4_dequant(const Fp4DequantArgs& p, cudaStream_t st);
@@ -444,6 +440,20 @@ struct Fp4SkinnyArgs {
 };
 cudaError_t g53_fp4_skinny(const Fp4SkinnyArgs& p, cudaStream_t st);
 
+// y[M, N] (mode) = x[M, K] bf16 @ W4[N, K]^T, the weights widened inside the kernel (fp4_exact.cu).  x: 16-byte aligned rows,
+// ldx >= K.  GEMV_SWIGLU as above
+struct Fp4ExactArgs {
+  const __nv_bfloat16* x; int64_t ldx;
+  const uint8_t* codes; const uint8_t* scales; const float* row_scale;
+  int nv;
+  void* y; int64_t ldy;
+  int M, N, K;
+  int width;
+  int mode;
+  float limit;
+};
+cudaError_t g53_fp4_exact(const Fp4ExactArgs& p, cudaStream_t st);
+
 // y[M, N] (mode) = A4[M, K] @ W4[N, K]^T on the block-scaled tensor-core path (fp4_gemm.cu).  out_* (GEMV_SWIGLU): the
 // activations are written as a 4-bit image [M, width] with the row scale 2^h_exp (nvfp4)
 struct Fp4GemmArgs {
@@ -459,8 +469,7 @@ struct Fp4GemmArgs {
   int vec;                             // set by the launcher: 16-byte epilogue stores allowed
 };
 cudaError_t g53_fp4_gemm(const Fp4GemmArgs& p, cudaStream_t st);
-// the current device's error word of the large-M kernels (bounded waits)
-cudaError_t g53_fp4_gemm_error_word(int** word);
 // first error code recorded on the current device by a bounded wait of these kernels (0: none); clears it
 cudaError_t g53_fp4_skinny_error(int* code);
+cudaError_t g53_fp4_exact_error(int* code);
 cudaError_t g53_fp4_gemm_error(int* code);

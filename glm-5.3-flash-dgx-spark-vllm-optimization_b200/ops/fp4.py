@@ -5,7 +5,7 @@ Formats (``FORMATS``); an element is its e2m1 code (0, .5, 1, 1.5, 2, 3, 4, 6 an
 times (nvfp4) its row's scale:
 
 * ``"nvfp4"``: blocks of 16 along K with an e4m3 scale, and a power of two per row (the smallest 2^k with the row's
-  largest magnitude <= 448 * 6 * 2^k); 4.5 bits per element.
+  largest magnitude <= 448 * 6 * 2^k, at least 2^-100); 4.5 bits per element.
 * ``"mxfp4"``: blocks of 32 along K with a power-of-two scale (the smallest 2^e with the block's largest magnitude <=
   6 * 2^e, so nothing saturates); 4.25 bits per element.
 
@@ -18,11 +18,14 @@ must not be rewritten while a call that reads them runs.
 
 Row counts and numerics of ``linear4`` / ``mlp4``:
 
-* up to 16 rows: exact bf16 activations (W4A16), one pass over the 4-bit weights on the small-M kernel;
-* more rows, ``act4=False``: exact activations too; up to 63 rows in passes of 16, from 64 rows the weights are widened
-  to bf16 (exact) for the tcgen05 GEMM;
-* more rows, ``act4=True``: activations are quantised per row to the weights' format and multiplied on the block-scaled
-  tensor cores (W4A4).
+* ``act4=False``, and up to 16 rows always: bf16 activations (W4A16).  Up to 96 rows each is expanded into 4-bit terms
+  for the 4-bit tensor cores, which leaves out at most 2^-22 of the largest magnitude of its block of 16 (nvfp4) or 32
+  (mxfp4) columns, in nvfp4 2^-39 of the row's where that is more; with more rows the weights are widened to bf16 inside
+  the product, exactly.  A row's result thus does not depend on the other rows, but its last bits on their number;
+* ``act4=True``, more than 16 rows: activations are quantised per row to the weights' format and multiplied on the
+  block-scaled tensor cores (W4A4).
+
+Sums are fp32 and added in a fixed order.
 """
 
 from __future__ import annotations

@@ -33,7 +33,7 @@ def scales(x, fmt, bound=None):
     if fmt == "mxfp4":
         return ceil_pow2(amax / 6)
     top = amax.amax(1, keepdim=True) if bound is None else x.new_full((x.shape[0], 1, 1), bound)
-    row = ceil_pow2(top / (448 * 6))
+    row = ceil_pow2(top / (448 * 6)).clamp_min(2.0 ** -100)
     return e4m3(torch.where(row > 0, amax / torch.where(row > 0, row, 1.0) / 6, 0.0)) * row
 
 
@@ -247,6 +247,83 @@ def test_linear_exact_activations_above_16_rows(fmt, m):
     assert ((y.double() - ref).abs() <= tol + half(BF) * (ref.abs() + tol)).all()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n,k", [(96, 70, 544), (97, 1, 32), (97, 129, 4128), (112, 257, 96), (256, 128, 2080), (257, 385, 544),
+                                   (300, 640, 12288), (512, 200, 1024), (513, 130, 1056), (1025, 300, 320), (1100, 20000, 96),
+                                   (2500, 1000, 160)])
+def test_linear_exact_activations_many_rows(fmt, m, n, k):
+    """Both sides of the row counts and widths where the product changes its shape: groups of rows, one or two mma, a split
+    of K over a cluster, an odd number of 128-row blocks."""
+    x, w = acts(m, k, m), weight(n, k, n)
+    w4, wq = fp4.quantize4(w, fmt), quant(w, fmt)
+    ref = x.double() @ wq.t()
+    tol = sums_tol(x.double(), wq) + act_tol(x.double(), wq, fmt)
+    out = torch.full((m + 2, n + 5), 5.0, dtype=F32, device="cuda")
+    y = fp4.linear4(x, w4, out[1:m + 1, 2:n + 2], K.GEMV_F32)
+    assert ((y.double() - ref).abs() <= tol).all()
+    got = y.clone()
+    out[1:m + 1, 2:n + 2] = 5.0
+    assert (out == 5.0).all()
+    assert torch.equal(fp4.linear4(x, w4, torch.empty(m, n, dtype=BF, device="cuda")), got.to(BF))
+    acc = torch.randn(m, n, device="cuda")
+    assert torch.equal(fp4.linear4(x, w4, acc.clone(), K.GEMV_F32_ACC), acc + got)
+    fp4.check_errors()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_linear_many_rows_magnitudes_and_views(fmt):
+    n, k, m = 200, 576, 140
+    src = weight(n, k, 2)
+    src[3] = 0
+    src[5] *= 2.0 ** 40
+    src[6] *= 2.0 ** -40
+    src[7] *= 2.0 ** -100
+    src[8] *= 2.0 ** 120
+    w4, wq = fp4.quantize4(src, fmt), quant(src, fmt)
+    big = acts(2 * m, 700, 4)
+    big[4] *= 2.0 ** -60
+    big[6] = 0
+    for off in (0, 1, 8):
+        x = big[::2, off:off + k]
+        ref = x.double() @ wq.t()
+        tol = sums_tol(x.double(), wq) + act_tol(x.double(), wq, fmt)
+        # products are summed 2^-8 lower in nvfp4: one below 2^-126 may lose what lies under 2^-149
+        tol += k * 2.0 ** -141
+        y = fp4.linear4(x, w4, torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32)
+        assert ((y.double() - ref).abs() <= tol).all()
+    one = acts(1, k, 6).expand(m, k)                    # the same row again and again
+    y = fp4.linear4(one, w4, torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32)
+    assert torch.equal(y, y[:1].expand(m, n))
+    assert torch.equal(y, fp4.linear4(one.contiguous(), w4, torch.empty_like(y), K.GEMV_F32))
+    x = acts(m, k, 9)
+    x[1, 7], x[130, 9] = math.inf, math.nan
+    y = fp4.linear4(x, w4, torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32)
+    fine = torch.ones(m, dtype=torch.bool, device="cuda")
+    fine[1] = fine[130] = False
+    assert torch.isfinite(y[fine]).all()
+    assert not torch.isfinite(y[1]).any() and torch.isnan(y[130]).all()
+
+
+def test_linear_takes_every_scale():
+    """Imported images: every code under every finite scale, through each product that keeps activations exact."""
+    for fmt in FMTS:
+        nv = fmt == "nvfp4"
+        n, k = 256, 256
+        src = fp4.quantize4(weight(n, k, 1), fmt)
+        codes = torch.arange(256, device="cuda", dtype=torch.uint8).repeat(src.codes.numel() // 256)
+        sc = torch.arange(src.scales.numel(), device="cuda") % 256
+        # finite, and with a sum of products inside fp32
+        sc = torch.where((sc & 127) == 127, 1, sc & 127) if nv else sc.clamp(0, 240)
+        m4 = fp4.Matrix4.from_parts(codes, sc.to(torch.uint8), torch.ones_like(src.row_scale) if nv else None, n, k, fmt)
+        w = fp4.dequantize4(m4, F32).double()
+        for m in (1, 40, 100, 300):
+            x = torch.ones(m, k, dtype=BF, device="cuda")
+            x[:, ::3] = -0.5
+            y = fp4.linear4(x, m4, torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32)
+            ref, tol = x.double() @ w.t(), sums_tol(x.double(), w) + k * 2.0 ** -126
+            assert ((y.double() - ref).abs() <= tol).all(), (fmt, m)
+
+
 # ------------------------------------------------------------------------------------- linear, 4-bit activations
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,n,k", [(17, 8, 32), (64, 128, 64), (100, 100, 96), (65, 20000, 96), (128, 200, 4128), (127, 4096, 96), (128, 256, 256), (129, 257, 288),
@@ -321,7 +398,8 @@ def h_slack(h, err, fmt, bound):
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,k,width,n", [(1, 4096, 2048, 512), (8, 512, 96, 40), (16, 288, 1536, 200), (5, 64, 32, 1),
                                          (33, 256, 160, 128), (64, 512, 96, 40), (150, 256, 1536, 200), (257, 512, 96, 40),
-                                         (300, 256, 1536, 200)])
+                                         (300, 256, 1536, 200), (97, 2080, 96, 40), (520, 1024, 160, 300),
+                                         (1040, 256, 2048, 130)])
 def test_mlp_exact_activations(fmt, m, k, width, n):
     limit = 2.0
     x, gate, up, down = acts(m, k, m), weight(width, k, 1), weight(width, k, 2), weight(n, width, 3)
@@ -389,7 +467,7 @@ def test_mlp_without_a_clamp():
 
 # ---------------------------------------------------------------------------------------- graphs, streams, reuse
 @pytest.mark.parametrize("m,act4", [(3, False), (12, False), (30, False), (90, False), (90, True),
-                                    (200, True), (270, False)])
+                                    (200, True), (270, False), (600, False)])
 def test_graph_replay_and_streams(m, act4):
     """Quantise, project and run the block as one captured graph, replayed on new inputs, beside eager calls on another
     stream: all the same bits."""
