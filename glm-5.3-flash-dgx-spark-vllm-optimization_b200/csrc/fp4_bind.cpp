@@ -20,8 +20,8 @@ using OptT = c10::optional<Tensor>;
 constexpr int64_t kTileRows = 128, kTileK = 256, kTileBytes = 16384;
 constexpr int64_t kFourRows = 16;      // rows above which act4 quantises the activations
 constexpr int64_t kFewRows = 96;       // rows up to which exact activations are expanded into 4-bit terms (24576 x 4096: 96 rows
-                                       // 48 us, 57 widened; 112 rows 67, 57.  4096 x 4096: 96 rows 16.3, 16.7; 112 rows 18.0,
-                                       // 16.9.  A 4096 x 12288 weight would gain from 64 rows on, 4096 x 2048 from 160)
+                                       // 48 us, 55 widened; 112 rows 67, 56.  4096 x 4096: 96 rows 15.9, 15.8; 112 rows 18.0,
+                                       // 16.4.  A 4096 x 12288 weight would gain from 64 rows on)
 constexpr int64_t kFour = 128;         // rows up to which 4-bit activations go through the small-M kernel (24576 x 4096: 100 rows
                                        // 28.8 us, 36.3 on the GEMM; 200 rows 42.6, 35.5)
 

@@ -5,20 +5,23 @@
 // A pair of CTAs (tcgen05.mma kind::f16, cta_group::2) takes 256 rows of W, 128 each, x up to 512 rows of X (the mma's
 // columns, one or two mma wide), and a slice of K; a cluster of CL pairs shares a tile.  Of X each CTA fetches one half: the
 // re-reading of X by every block of W is what the L2 has to carry (a CTA on its own with all of it: 300 rows x 24576 x 4096
-// 111 us, 73 in pairs).  Warp roles:
+// 111 us, 72 in pairs).  Warp roles:
 //   warp 0     X tiles (64 columns, TMA with 128-byte swizzle) into a ring
 //   warp 1     allocates TMEM; one thread of the pair's first CTA issues four mma (K = 16) per stage and column half; that of
 //              the second passes on that its stage is ready
 //   warp 2     4-bit tiles (128 x 256: one contiguous cp.async.bulk of codes, one of scales) into a second ring
 //   warps 3-18 widen, in two sets of 8 that take the ring's stages in turn: a thread half a row of 64 columns (one 16-byte
 //              chunk), written as the swizzled operand; then the epilogue
-// Bound: a stage takes the tensor core 2 clocks per row of X (512 rows: 1007 measured) and the widening warps about 600 (64
-// rows; 850 with one set, no better with three), so from 300 rows on the mma sets the pace and below the widening.  Writing
-// the widened weights to memory for a bf16 product would cost 4 1/2 bytes of traffic per weight instead of 9/16: 300 rows
-// x 24576 x 4096 121 us (73 here), 300 x 4096 x 12288 101 (44), 2000 x 24576 x 4096 354 (306), 8192 x 12288 x 4096 621 (618).
+// Bound: a stage takes the tensor core 2 clocks per row of X (512 rows: 1007 measured), and widening and the hand-over between
+// the roles about 640 (64 rows; 850 with one set of widening warps, no better with three; 420 with neither widening nor mma
+// nor copies), so from 320 rows on the mma sets the pace.  Writing the widened weights to memory for a bf16 product instead
+// costs 4 1/2 bytes of traffic per weight, not 9/16: 300 rows x 24576 x 4096 121 us (72 here), 300 x 4096 x 12288 101 (39),
+// 300 x 4096 x 4096 34.5 (22), 2000 x 24576 x 4096 354 (305); it came out ahead only at 8192 rows of a 4096 x 4096 weight,
+// 193 (217), where its epilogue overlaps the next tile.
 //
 // The slices of a cluster are written as fp32 to each CTA's shared memory and added in rank order by the rank that owns the
-// rows, so the result does not depend on timing.  Waits are bounded; one that runs out sets the error word, the roles stop
+// rows, so the result does not depend on timing (300 rows x 4096 x 4096: 22.1 us with the owner's loads all in flight, 26.8
+// with one at a time).  Waits are bounded; one that runs out sets the error word, the roles stop
 // issuing, wait for what they have in flight, every barrier is still reached and the TMEM is freed.
 #include <cuda.h>
 #include <algorithm>
@@ -39,7 +42,9 @@ constexpr int kExThreads = (kRoles + kWiden) * 32;
 constexpr int kWStages = 3;                           // 4-bit tiles in flight
 constexpr int kABytes = 128 * 128;                    // a stage's bf16 weights: 128 rows x 64
 
-constexpr int kPass = 256;                            // rows of X whose sums lie in shared memory at a time
+constexpr int kPass = 416;                            // rows of X whose sums lie in shared memory at a time,
+constexpr int kPartLd = 132;                          // 128 each, and 4 so that the same columns of rows share no banks
+constexpr int kMaxSplit = 3;                            // slices of K
 constexpr int kMaxCols = 512;                         // rows of X of a pair: all of TMEM
 
 struct ExPlan {
@@ -87,20 +92,52 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
   asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
                ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("{\n .reg .u32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n}\n"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
   return v;
 }
 
 __device__ __forceinline__ void ex_store(const Fp4ExactArgs& p, int64_t tok, int n, float v) {
   const int64_t off = tok * p.ldy + n;
-  if (p.mode == GEMV_BF16) {
+  if (p.mode == GEMV_BF16 || p.mode == GEMV_SWIGLU) {
     reinterpret_cast<__nv_bfloat16*>(p.y)[off] = f2bf(v);
   } else {
     float* y = reinterpret_cast<float*>(p.y) + off;
     *y = p.mode == GEMV_F32_ACC ? *y + v : v;
   }
+}
+
+// clamped SwiGLU, written so that a NaN stays one
+__device__ __forceinline__ float ex_gate(float g, float u, float limit) {
+  g = g > limit ? limit : g;
+  u = u > limit ? limit : u < -limit ? -limit : u;
+  return siluf_(g) * u;
+}
+
+// columns n .. n + 3 of a row of y, those below `end`
+__device__ __forceinline__ void ex_store4(const Fp4ExactArgs& p, int64_t tok, int n, int end, float4 v) {
+  if (p.vec && n + 4 <= end) {
+    const int64_t off = tok * p.ldy + n;
+    if (p.mode == GEMV_BF16 || p.mode == GEMV_SWIGLU) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+      *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.y) + off) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+      float4* y = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + off);
+      if (p.mode == GEMV_F32_ACC) {
+        const float4 t = *y;
+        v.x += t.x; v.y += t.y; v.z += t.z; v.w += t.w;
+      }
+      *y = v;
+    }
+    return;
+  }
+  const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < end) ex_store(p, tok, n + i, o[i]);
 }
 
 template <bool NV>
@@ -202,23 +239,36 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
           if (++s == pl.stages) { s = 0; ph ^= 1; }
         }
       } else {
+        // The pace of the whole kernel hangs on this thread, which shares its scheduler with the widening warps: the next
+        // stage's barrier is looked at before this stage's mma are issued (a look takes about 115 clocks)
         const int cols = pl.ncol / pl.mmas;
         const uint32_t id = tc::idesc(1, cols, 256);
         const uint16_t both = (uint16_t)(3u << crank);
+        const uint64_t a0 = tc::desc_sw128(tc::saddr(ring));            // descriptors count in units of 16 bytes
+        const uint32_t step = (uint32_t)pl.stage_bytes >> 4, b_off = kABytes >> 4, b2_off = b_off + (uint32_t)cols * 4;
         uint32_t acc = 0;
+        uint64_t a = a0;
+        bool ready = tc::bar_try(&full[0], 0);
         for (int st = 0; st < n_st; ++st) {
-          if (!tc::bar_wait(&full[s], ph, fail, &g_exact_err, 7)) { ok = false; break; }
+          if (!ready && !tc::bar_wait(&full[s], ph, fail, &g_exact_err, 7)) { ok = false; break; }
           tc::fence_after();
-          const uint32_t sa = tc::saddr(ring + s * pl.stage_bytes);
-          const uint64_t a = tc::desc_sw128(sa), b = tc::desc_sw128(sa + kABytes), b2 = tc::desc_sw128(sa + kABytes + cols * 64);
+          const int at = s;
+          const uint64_t d = a;
+          if (++s == pl.stages) {
+            s = 0;
+            ph ^= 1;
+            a = a0;
+          } else {
+            a += step;
+          }
+          ready = tc::bar_try(&full[s], ph);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            mma_pair(tmem, a + 2 * k, b + 2 * k, id, acc);             // 32 bytes on in the descriptors' units of 16
-            if (pl.mmas == 2) mma_pair(tmem + cols, a + 2 * k, b2 + 2 * k, id, acc);
+            mma_pair(tmem, d + 2 * k, d + (b_off + 2 * k), id, acc);
+            if (pl.mmas == 2) mma_pair(tmem + cols, d + 2 * k, d + (b2_off + 2 * k), id, acc);
             acc = 1;
           }
-          commit_pair(&empty[s], both);
-          if (++s == pl.stages) { s = 0; ph ^= 1; }
+          commit_pair(&empty[at], both);
         }
         if (ok) {
           commit_pair(&tfull, both);
@@ -294,7 +344,7 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
           if (!meet) {
             if (n < p.N) ex_store(p, x0 + c0 + i, n, v[i] * rs);
           } else {
-            part[(c0 + i - cb) * 128 + r] = v[i] * rs;
+            part[(c0 + i - cb) * kPartLd + r] = v[i] * rs;
           }
         }
       }
@@ -309,30 +359,35 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
       __syncthreads();
     }
     if (warp >= kRoles) {
-      const int et = threadIdx.x - kRoles * 32, pairs = (64 + CL - 1) / CL;
-      const int j_lo = rank * pairs, cnt = min(64, j_lo + pairs) - j_lo;
+      // a thread takes columns r .. r + 3 and r + 64 .. of one row of X: every load of the cluster's parts is on its way
+      // before the first is used
+      const int et = threadIdx.x - kRoles * 32, quads = (16 + CL - 1) / CL;
+      const int q_lo = rank * quads, cnt = min(16, q_lo + quads) - q_lo;
       const uint32_t base = tc::saddr(part);
-      for (int e = et; e < (ce - cb) * pairs; e += kWiden * 32) {
-        const int c = e / pairs, tok = x0 + cb + c, r = j_lo + e - c * pairs;
-        if (r >= j_lo + cnt) continue;
-        float v = 0.f, u = 0.f;
-        for (int k = 0; k < CL; ++k) {
-          uint32_t a = base + (c * 128 + r) * 4;
-          asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(a) : "r"(CL > 1 ? 2 * k + side : crank));
-          v += ld_cluster(a);
-          u += ld_cluster(a + 64 * 4);
-        }
-        const int n = nb * 128 + r;
+      for (int e = et; e < (ce - cb) * quads; e += kWiden * 32) {
+        const int c = e / quads, tok = x0 + cb + c, q = e - c * quads, r = (q_lo + q) * 4;
+        if (q >= cnt) continue;
+        const uint32_t at = base + (c * kPartLd + r) * 4;
+        float4 g[kMaxSplit], h[kMaxSplit];
+#pragma unroll
+        for (int k = 0; k < kMaxSplit; ++k)
+          if (k < CL) {
+            g[k] = ld_cluster4(at, CL > 1 ? 2 * k + side : crank);
+            h[k] = ld_cluster4(at + 64 * 4, CL > 1 ? 2 * k + side : crank);
+          }
+        float4 v = g[0], u = h[0];
+#pragma unroll
+        for (int k = 1; k < kMaxSplit; ++k)
+          if (k < CL) {
+            v.x += g[k].x; v.y += g[k].y; v.z += g[k].z; v.w += g[k].w;
+            u.x += h[k].x; u.y += h[k].y; u.z += h[k].z; u.w += h[k].w;
+          }
         if (swi) {
-          const int col = nb * 64 + r;
-          if (col >= p.width) continue;
-          // written so that a NaN stays one
-          v = v > p.limit ? p.limit : v;
-          u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
-          reinterpret_cast<__nv_bfloat16*>(p.y)[(int64_t)tok * p.ldy + col] = f2bf(siluf_(v) * u);
+          ex_store4(p, tok, nb * 64 + r, p.width, make_float4(ex_gate(v.x, u.x, p.limit), ex_gate(v.y, u.y, p.limit),
+                                                              ex_gate(v.z, u.z, p.limit), ex_gate(v.w, u.w, p.limit)));
         } else {
-          if (n < p.N) ex_store(p, tok, n, v);
-          if (n + 64 < p.N) ex_store(p, tok, n + 64, u);
+          ex_store4(p, tok, nb * 128 + r, p.N, v);
+          ex_store4(p, tok, nb * 128 + r + 64, p.N, u);
         }
       }
     }
@@ -374,7 +429,7 @@ static EncodeTiled encode_tiled() {
   return fn;
 }
 
-constexpr int kExBudget = 225 * 1024, kMaxSplit = 3, kMaxDev = 64;
+constexpr int kExBudget = 225 * 1024, kMaxDev = 64;
 
 // Stands in for the product in the question below: the runtime answers wrongly for a kernel that uses TMEM
 __global__ void __launch_bounds__(kExThreads, 1) ex_shape_kernel() {}
@@ -403,10 +458,10 @@ static cudaError_t ex_active(int dev, int cl, int* out) {
   return cudaSuccess;
 }
 
-// Shape: groups of rows of X and K split with the least time, in clocks.  A stage of 64 columns takes the widening (500) or
-// the mma (2 per row of X, and 60); a tile 7000 and 8 per row beside that, the exchange of a cluster 4000 and 12 per row.
-// Fitted to a sweep of both over 16 row counts from 64 to 8192 and seven weight sizes: the shape chosen is 2% from the best
-// of the sweep on average, 28% at worst.  An eighth of the clusters' room stays free, as one that has to wait doubles the time.
+// Shape: groups of rows of X and K split with the least time, in clocks.  A stage of 64 columns takes the warps and barriers
+// (600) or the mma (2 per row of X); a tile 9000 and 16 per row beside that, the exchange of a cluster 1000 and 8 per row.
+// Fitted to a sweep of both over 15 row counts from 97 to 4096 and six weight sizes: the shape chosen is 1% from the best of
+// the sweep on average, 14% at worst.  Room for one cluster stays free, as one that has to wait doubles the time.
 template <bool NV>
 static cudaError_t launch_exact(const Fp4ExactArgs& p, cudaStream_t st) {
   int dev = 0, sms = 0;
@@ -436,10 +491,10 @@ static cudaError_t launch_exact(const Fp4ExactArgs& p, cudaStream_t st) {
       int active = 0;
       e = ex_active(dev, cl, &active);
       if (e != cudaSuccess) return e;
-      if (cl > 1) active -= active / 8;
+      if (cl > 1) active = std::max(1, active - 1);
       const int64_t units = pairs * groups;
       const double t = (double)((units + active - 1) / active) *
-                       (per * 4.0 * std::max(500, 2 * ncol + 60) + 7000 + 8 * ncol + (cl > 1 ? 4000 + 12 * ncol : 0));
+                       (per * 4.0 * std::max(600, 2 * ncol) + 9000 + 16 * ncol + (cl > 1 ? 1000 + 8 * ncol : 0));
       if (b.CL == 0 || t < best) {
         best = t;
         b.CL = cl;
@@ -457,7 +512,7 @@ static cudaError_t launch_exact(const Fp4ExactArgs& p, cudaStream_t st) {
   b.stage_bytes = kABytes + b.ncol * 64;
   b.stages = std::min(8, (kExBudget - 1024 - kWStages * kWBytes) / b.stage_bytes);
   // the sums lie over both rings
-  const int smem = std::max(b.stages * b.stage_bytes + kWStages * kWBytes, std::min(b.ncol, kPass) * 512) + 1024;
+  const int smem = std::max(b.stages * b.stage_bytes + kWStages * kWBytes, std::min(b.ncol, kPass) * kPartLd * 4) + 1024;
 
   EncodeTiled fn = encode_tiled();
   if (!fn) return cudaErrorNotSupported;
@@ -499,7 +554,10 @@ cudaError_t g53_fp4_exact(const Fp4ExactArgs& p, cudaStream_t st) {
   if (p.M < 1 || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32) || (reinterpret_cast<uintptr_t>(p.x) & 15) || p.ldx % 8 ||
       p.ldx < p.K)
     return cudaErrorInvalidValue;
-  return p.nv ? fp4::launch_exact<true>(p, st) : fp4::launch_exact<false>(p, st);
+  Fp4ExactArgs q = p;
+  const bool half = p.mode == GEMV_BF16 || p.mode == GEMV_SWIGLU;
+  q.vec = (reinterpret_cast<uintptr_t>(p.y) & (half ? 7 : 15)) == 0 && p.ldy % 4 == 0;
+  return p.nv ? fp4::launch_exact<true>(q, st) : fp4::launch_exact<false>(q, st);
 }
 
 cudaError_t g53_fp4_exact_error(int* code) {

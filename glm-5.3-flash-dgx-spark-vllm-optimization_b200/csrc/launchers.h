@@ -451,6 +451,7 @@ struct Fp4ExactArgs {
   int width;
   int mode;
   float limit;
+  int vec;                             // set by the launcher: wide stores allowed
 };
 cudaError_t g53_fp4_exact(const Fp4ExactArgs& p, cudaStream_t st);
 
