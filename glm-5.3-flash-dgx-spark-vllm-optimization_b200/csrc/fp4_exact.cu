@@ -26,6 +26,7 @@
 #include <cuda.h>
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include "fp4.cuh"
 #include "fp4_tc.cuh"
 #include "launchers.h"
@@ -105,7 +106,7 @@ __device__ __forceinline__ void ex_store(const Fp4ExactArgs& p, int64_t tok, int
     reinterpret_cast<__nv_bfloat16*>(p.y)[off] = f2bf(v);
   } else {
     float* y = reinterpret_cast<float*>(p.y) + off;
-    *y = p.mode == GEMV_F32_ACC ? *y + v : v;
+    *y = p.mode == GEMV_F32_ACC ? __ldcg(y) + v : v;
   }
 }
 
@@ -127,7 +128,7 @@ __device__ __forceinline__ void ex_store4(const Fp4ExactArgs& p, int64_t tok, in
     } else {
       float4* y = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + off);
       if (p.mode == GEMV_F32_ACC) {
-        const float4 t = *y;
+        const float4 t = __ldcg(y);
         v.x += t.x; v.y += t.y; v.z += t.z; v.w += t.w;
       }
       *y = v;
@@ -551,7 +552,7 @@ static cudaError_t launch_exact(const Fp4ExactArgs& p, cudaStream_t st) {
 using namespace g53;
 
 cudaError_t g53_fp4_exact(const Fp4ExactArgs& p, cudaStream_t st) {
-  if (p.M < 1 || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32) || (reinterpret_cast<uintptr_t>(p.x) & 15) || p.ldx % 8 ||
+  if (p.M < 1 || p.M > INT_MAX - fp4::kMaxCols || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32) || (reinterpret_cast<uintptr_t>(p.x) & 15) || p.ldx % 8 ||
       p.ldx < p.K)
     return cudaErrorInvalidValue;
   Fp4ExactArgs q = p;

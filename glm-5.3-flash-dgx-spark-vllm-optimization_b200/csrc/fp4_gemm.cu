@@ -80,7 +80,7 @@ __device__ __forceinline__ void store32(const Fp4GemmArgs& p, int row, int nb, f
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (nb + i + j < p.N) v[i + j] *= rs * p.b_row[nb + i + j];
+          if (nb + i + j < p.N) v[i + j] *= rs * __ldcg(p.b_row + nb + i + j);
       }
     }
   }
@@ -112,7 +112,7 @@ __device__ __forceinline__ void store32(const Fp4GemmArgs& p, int row, int nb, f
     for (int c = 0; c < 8; ++c) {
       float4 o = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
       if (acc) {
-        const float4 t = reinterpret_cast<const float4*>(y)[c];
+        const float4 t = __ldcg(reinterpret_cast<const float4*>(y) + c);
         o.x += t.x; o.y += t.y; o.z += t.z; o.w += t.w;
       }
       reinterpret_cast<float4*>(y)[c] = o;
@@ -120,7 +120,7 @@ __device__ __forceinline__ void store32(const Fp4GemmArgs& p, int row, int nb, f
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if (nb + i < p.N) y[i] = acc ? y[i] + v[i] : v[i];
+      if (nb + i < p.N) y[i] = acc ? __ldcg(y + i) + v[i] : v[i];
   }
 }
 
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
       tc::fence_after();
       const int row = (mt * kG + rank) * 128 + quad * 32 + lane;
       const bool live = row < p.M;
-      const float rs = p.a_row && live ? p.a_row[row] : p.a_const;
+      const float rs = p.a_row && live ? __ldcg(p.a_row + row) : p.a_const;
       const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + buf * C::kBuf;
       auto release = [&]() {
         tc::fence_before();

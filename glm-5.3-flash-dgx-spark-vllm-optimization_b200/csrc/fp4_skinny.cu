@@ -213,7 +213,7 @@ __device__ __forceinline__ void store1(const Fp4SkinnyArgs& p, int tok, int n, f
     reinterpret_cast<__nv_bfloat16*>(p.y)[off] = f2bf(v);
   } else {
     float* y = reinterpret_cast<float*>(p.y) + off;
-    *y = p.mode == GEMV_F32_ACC ? *y + v : v;
+    *y = p.mode == GEMV_F32_ACC ? __ldcg(y) + v : v;
   }
 }
 // four values into the shared memory of a CTA of the cluster, counted on its barrier (both addresses mapped to that CTA)

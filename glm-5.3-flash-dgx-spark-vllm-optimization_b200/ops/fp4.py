@@ -57,6 +57,8 @@ class Matrix4:
 
     @classmethod
     def from_parts(cls, codes, scales, row_scale, rows: int, k: int, fmt: str) -> "Matrix4":
+        """A matrix from arrays in the layout of ``codes``, ``scales`` and ``row_scale``.  Codes and scales of the columns
+        from k up to a multiple of 256 must be 0, as ``quantize4`` leaves them; every row scale a power of two."""
         return cls(_ext.require().Matrix4(codes, scales, row_scale, rows, k, _nv(fmt)))
 
     @property

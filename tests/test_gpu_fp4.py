@@ -516,6 +516,25 @@ def test_weights_written_just_before_their_product():
         assert torch.equal(y, fp4.linear4(x, w4, torch.empty_like(y), K.GEMV_F32))
 
 
+@pytest.mark.parametrize("m,act4", [(3, False), (60, False), (60, True), (150, False), (150, True), (700, False)])
+def test_sums_added_call_after_call(m, act4):
+    """Products that add into y right behind one another (rows of odd length: two CTAs share sectors of y) see each other's
+    sums."""
+    n, k = 389, 512
+    w4 = fp4.quantize4(weight(n, k, 4), "nvfp4")
+    xs = [acts(m, k, s) for s in range(4)]
+
+    def chain(wait):
+        y = torch.zeros(m, n, device="cuda")
+        for i in range(40):
+            fp4.linear4(xs[i % 4], w4, y, K.GEMV_F32_ACC, act4=act4)
+            if wait:
+                torch.cuda.synchronize()
+        return y
+    want = chain(True)
+    assert all(torch.equal(chain(False), want) for _ in range(5))
+
+
 def test_first_calls_inside_a_capture():
     """In a fresh process, each product's first launch may be a captured one."""
     import os
