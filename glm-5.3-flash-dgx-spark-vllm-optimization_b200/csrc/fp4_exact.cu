@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
     if (live) live = tc::warp_wait(&tfull, 0, fail, &g_exact_err, 6);
     tc::fence_after();
   }
-  // ---- sums: a thread holds one row of W; those of the cluster meet in shared memory
-  const bool swi = p.mode == GEMV_SWIGLU, meet = CL > 1 || swi;
+  // ---- sums: a thread holds one row of W; they meet in shared memory, with those of the cluster
+  const bool swi = p.mode == GEMV_SWIGLU;
   for (int cb = 0; cb < M; cb += kPass) {
     const int ce = min(M, cb + kPass);
     if (warp >= kRoles) {
@@ -342,15 +342,10 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
         for (int i = 0; i < 32; ++i) {
           if (c0 + i >= ce) break;
           if (NV) v[i] *= 256.f;
-          if (!meet) {
-            if (n < p.N) ex_store(p, x0 + c0 + i, n, v[i] * rs);
-          } else {
-            part[(c0 + i - cb) * kPartLd + r] = v[i] * rs;
-          }
+          part[(c0 + i - cb) * kPartLd + r] = v[i] * rs;
         }
       }
     }
-    if (!meet) continue;
     // every CTA of the cluster has its sums in shared memory
     if (CL > 1) {
       __syncwarp();
@@ -552,7 +547,8 @@ static cudaError_t launch_exact(const Fp4ExactArgs& p, cudaStream_t st) {
 using namespace g53;
 
 cudaError_t g53_fp4_exact(const Fp4ExactArgs& p, cudaStream_t st) {
-  if (p.M < 1 || p.M > INT_MAX - fp4::kMaxCols || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32) || (reinterpret_cast<uintptr_t>(p.x) & 15) || p.ldx % 8 ||
+  if (p.M < 1 || p.M > INT_MAX - fp4::kMaxCols || p.N < 1 || p.K < 16 || p.K % (p.nv ? 16 : 32) ||
+      (reinterpret_cast<uintptr_t>(p.x) & 15) || p.ldx % 8 ||
       p.ldx < p.K)
     return cudaErrorInvalidValue;
   Fp4ExactArgs q = p;
