@@ -1,4 +1,5 @@
-// Small-M product with 4-bit weights: Y[M, N] = X[M, K] @ W4[N, K]^T for M <= 32 rows of 16-bit activations (W4A16).
+// Small-M product with 4-bit weights: Y[M, N] = X[M, K] @ W4[N, K]^T for up to 96 rows of 16-bit activations (W4A16, in groups of
+// 16 or 32) or up to 128 4-bit rows.
 //
 // A decode projection reads every weight byte once, so HBM is the floor: 9/16 (17/32) byte per weight.  Widening the
 // weights to f16 operands on the CUDA cores cannot keep up with that (built first: 390 instructions per warp and 32 x 128
