@@ -218,13 +218,13 @@ void skinny(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t width, i
   ok(g53_fp4_skinny(a, stream()), "fp4_skinny");
 }
 
-// 4-bit activations, few rows; `factor`: the row scale of all rows, where x has none of its own
-void skinny4(const Matrix4& x, float factor, const Matrix4& w, const Tensor& y, int64_t mode) {
+// 4-bit activations, few rows, with their row scales, or (null: x's own are not set, or there are none) one for all rows
+void skinny4(const Matrix4& x, const float* row_scale, float one, const Matrix4& w, const Tensor& y, int64_t mode) {
   Fp4SkinnyArgs a = skinny_args(x.rows, w, y, 0, mode, 0.0);
   a.x_codes = x.codes;
   a.x_scales = x.scales;
-  a.x_factor = factor == 1.f ? x.row_scale : nullptr;
-  a.x_const = factor;
+  a.x_factor = row_scale;
+  a.x_const = one;
   a.terms = 1;
   ok(g53_fp4_skinny(a, stream()), "fp4_skinny");
 }
@@ -277,7 +277,7 @@ void linear(const Tensor& x, const Matrix4& w, const Tensor& y, int64_t mode, bo
   if (M > kFourRows && act4) {
     const Matrix4 a = quantize(x, w.nv);
     if (M <= kFour) {
-      skinny4(a, 1.f, w, y, mode);
+      skinny4(a, a.row_scale, 1.f, w, y, mode);
       return;
     }
     Fp4GemmArgs p = gemm_args(a, w, mode);
@@ -325,7 +325,7 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
     ok(g53_fp4_gemm(p, stream()), "fp4_gemm");
     const float factor = gu.nv ? std::ldexp(1.f, p.h_exp) : 1.f;
     if (M <= kFour) {
-      skinny4(h, factor, down, y, mode);
+      skinny4(h, nullptr, factor, down, y, mode);
       return;
     }
     Fp4GemmArgs d = gemm_args(h, down, mode);
