@@ -307,9 +307,10 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
   check_xy(x, gu, y, down.rows, mode, "mlp4");
   TORCH_CHECK(limit > 0, "mlp4: limit must be positive (infinity: no clamp)");
   const int64_t M = x.size(0);
-  const float l2 = (float)limit * (float)limit;
+  // bounds |h|: |u| <= limit, and silu(min(g, limit)) lies in [-0.27847, limit]
+  const float h_max = std::max((float)limit, 0.2785f) * (float)limit;
   const bool four = act4 && M > kFourRows;
-  TORCH_CHECK(!four || !gu.nv || (std::isfinite(l2) && l2 >= 1e-30f),
+  TORCH_CHECK(!four || !gu.nv || (std::isfinite(h_max) && h_max >= 1e-30f),
               "mlp4: 4-bit nvfp4 activations need a finite limit (their row scale comes from it)");
   if (M == 0) return;
   const c10::cuda::CUDAGuard guard(x.device());
@@ -321,7 +322,7 @@ void mlp(const Tensor& x, const Matrix4& gu, const Matrix4& down, const Tensor& 
     p.width = (int)W;
     p.out_codes = h.codes;
     p.out_scales = h.scales;
-    p.h_exp = gu.nv ? row_exp(l2) : 0;
+    p.h_exp = gu.nv ? row_exp(h_max) : 0;
     ok(g53_fp4_gemm(p, stream()), "fp4_gemm");
     const float factor = gu.nv ? std::ldexp(1.f, p.h_exp) : 1.f;
     if (M <= kFour) {

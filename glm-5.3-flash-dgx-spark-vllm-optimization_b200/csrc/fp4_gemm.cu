@@ -24,8 +24,8 @@
 // GEMV_SWIGLU: W4 is a gate/up image (per 128-row block 64 gate rows, then their 64 up rows); the epilogue forms
 // silu(min(g, L)) * clip(u, -L, L) in fp32 and quantises it in place: a thread holds 32 consecutive activations of one row,
 // a whole 16-byte chunk of the 4-bit image that the down projection reads.  The nvfp4 row scale cannot wait for the row's
-// maximum (other CTAs hold the rest of the row), so it is the one that fits L * L, the largest possible activation; the
-// e4m3 block scales then have 2^15 of range below it.
+// maximum (other CTAs hold the rest of the row), so it is the one that fits max(L, 0.2785) * L, which no activation exceeds
+// (silu's lowest value is -0.27847); the e4m3 block scales keep their precision down to about 2^-14 of that.
 //
 // Waits are bounded; a timeout sets the error word, the roles stop issuing, wait for what they have in flight, and the
 // TMEM is freed.

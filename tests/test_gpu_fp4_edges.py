@@ -44,3 +44,11 @@ def check_mlp_act4(fmt, m, k, width, n, limit):
 @pytest.mark.parametrize("limit", [36.0, 40.0, 50.0, 51.84, 60.0])
 def test_mlp_4bit_activations_wide_limits(fmt, m, limit):
     check_mlp_act4(fmt, m, 256, 160, 72, limit)
+
+
+# below 0.2785 the gate's lowest value, -0.2785, is further out than the limit
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m", [17, 100, 200])
+@pytest.mark.parametrize("limit", [0.01, 0.1, 0.25, 0.28])
+def test_mlp_4bit_activations_small_limits(fmt, m, limit):
+    check_mlp_act4(fmt, m, 256, 160, 72, limit)
