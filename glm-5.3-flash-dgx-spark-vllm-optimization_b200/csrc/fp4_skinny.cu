@@ -25,8 +25,9 @@
 // of the cluster that owns the row (st.async into its shared memory, counted in bytes on its barrier: stores with a
 // cluster-scope release behind them took a microsecond) and finish the rows they own, adding in rank order: the result does
 // not depend on timing.  Two receive buffers alternate: a rank can only send block b + 2 after it received every rank's b +
-// 1, which each sent after it had finished reading b.  No barrier is needed at the end: a CTA leaves after it has received
-// all that is sent to it.
+// 1, and no thread of a rank sends of b + 1 before all of its warps have read b (a barrier of theirs: those that hold none of a
+// peer's rows send it nothing, so the arrival of b + 1 alone says nothing about them).  No barrier is needed at the end: a CTA
+// leaves after it has received all that is sent to it.
 //
 // Before griddepcontrol.wait only prefetches into L2 are issued: the weights may be what the previous kernel writes.
 // Waits are bounded; one that runs out sets the error word, and the CTA goes on without the main loop's waits but sends and
@@ -537,6 +538,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
             if (tok + i < M) store1(p, x0 + tok + i, n, vs[i] * sc);
         }
       }
+      if (CL > 1 && u + pl.clusters < pl.units) sk_sync();   // this block is read: its sums of the next may go out
     }
   }
   tc::fence_before();

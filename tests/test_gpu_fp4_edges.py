@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from glm53.ops import fp4
-from test_gpu_fp4 import F32, FMTS, acts, gated, h_slack, quant, sums_tol, weight
+from glm53.ops import kernels as K
+from test_gpu_fp4 import F32, FMTS, act_tol, acts, gated, h_slack, quant, sums_tol, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +53,19 @@ def test_mlp_4bit_activations_wide_limits(fmt, m, limit):
 @pytest.mark.parametrize("limit", [0.01, 0.1, 0.25, 0.28])
 def test_mlp_4bit_activations_small_limits(fmt, m, limit):
     check_mlp_act4(fmt, m, 256, 160, 72, limit)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 38400, 6144), (4, 38400, 6144), (16, 38400, 6144), (96, 6400, 12288)])
+def test_linear_repeats_itself_over_many_row_blocks(m, n, k):
+    """Clusters that share blocks of weight rows and go through three or more: the exchange of a block must not reach a rank
+    that still reads the one two before it."""
+    fmt = "mxfp4"
+    x, w4 = acts(m, k, m), fp4.quantize4(weight(n, k, 3), fmt)
+    y = fp4.linear4(x, w4, torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32)
+    for _ in range(50):
+        assert torch.equal(fp4.linear4(x, w4, torch.empty_like(y), K.GEMV_F32), y)
+    some = torch.arange(0, n, 97, device="cuda")
+    wq = fp4.dequantize4(w4, F32)[some].double()
+    tol = sums_tol(x.double(), wq) + act_tol(x.double(), wq, fmt)
+    assert ((y[:, some].double() - x.double() @ wq.t()).abs() <= tol).all()
+    fp4.check_errors()
