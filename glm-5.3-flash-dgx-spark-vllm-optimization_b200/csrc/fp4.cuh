@@ -94,6 +94,19 @@ __device__ __forceinline__ uint32_t nv_scale(float amax_scaled) {
   return (uint32_t)v.__x;
 }
 
+// A row scale rs = a * b for a sum v that another row scale t (2^-100 .. 2^119) applies to, too: v * (a * t) * b is right
+// wherever v * rs * t is a value of fp32.  rs * t itself may not be one (2^-76 * 2^-76), nor v * rs (2^30 * 2^107, t = 2^-15).  a is
+// kept in [2^-36, 2^8], so a * t is a power of two of fp32, and for |v| < 2^44 nothing overflows that comes back into range, or
+// loses bits that the result has.  b is 1 for rows whose largest magnitude lies between 2^-24 and 2^19.  A NaN stays one.
+struct RowScale {
+  float a, b;
+};
+__device__ __forceinline__ RowScale split_scale(float rs) {
+  if (rs > 0x1p8f) return {0x1p8f, rs * 0x1p-8f};
+  if (rs < 0x1p-36f) return {0x1p-36f, rs * 0x1p36f};
+  return {rs, 1.f};
+}
+
 // x * inv on the grid of 2^-15, for |x * inv| < 8 and inv the rounded reciprocal of a block scale s (times a power of
 // two).  For x of at most 11 significant bits (bf16, f16) and s of at most 4, x / s either equals a border between two
 // codes (a multiple of 1/4) or is at least 2^-11 of it, so 2^-13, away: the error that the reciprocal adds (below 2^-20) is

@@ -87,20 +87,22 @@ __device__ __forceinline__ void transpose32(float (&v)[32]) {
 // 32 columns nb.. of the warp's 32 rows, `row` that of this lane.  16-byte aligned rows are stored by their lanes; others go
 // out a row at a time, 32 lanes side by side (2786 x 3916 x 1728 in bf16: 53 us, 151 with a lane's own row element by
 // element, which only the last columns of aligned rows take).
-__device__ __forceinline__ void store32(const Fp4GemmArgs& p, int row, int nb, float rs, float (&v)[32]) {
+__device__ __forceinline__ void store32(const Fp4GemmArgs& p, int row, int nb, RowScale rs, float (&v)[32]) {
   const bool full = nb + 32 <= p.N, acc = p.mode == GEMV_F32_ACC;
   if (p.b_row) {
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       if (full) {
         const float4 t = __ldcg(reinterpret_cast<const float4*>(p.b_row + nb + i));
-        v[i] *= rs * t.x; v[i + 1] *= rs * t.y; v[i + 2] *= rs * t.z; v[i + 3] *= rs * t.w;
+        v[i] *= rs.a * t.x; v[i + 1] *= rs.a * t.y; v[i + 2] *= rs.a * t.z; v[i + 3] *= rs.a * t.w;
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (nb + i + j < p.N) v[i + j] *= rs * __ldcg(p.b_row + nb + i + j);
+          if (nb + i + j < p.N) v[i + j] *= rs.a * __ldcg(p.b_row + nb + i + j);
       }
     }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= rs.b;
   }
   if (!p.vec) {
     transpose32(v);
@@ -176,8 +178,10 @@ __device__ __forceinline__ void swiglu32(const Fp4GemmArgs& p, int row, int j0, 
     for (int k = 0; k < 4; ++k) {
       float g = v[i + k], w = u[i + k];
       if constexpr (NV) {
-        g *= rs * gs[k];
-        w *= rs * us[k];
+        // one scale after the other: their product may leave fp32 (and 0 * inf is NaN).  In this order a sum overflows on the
+        // way only where the weights' scale is above 2^90; RowScale's third product would cost the epilogue 2%
+        g = g * gs[k] * rs;
+        w = w * us[k] * rs;
       }
       g = g > L ? L : g;                              // written so that a NaN stays one
       w = w > L ? L : w < -L ? -L : w;
@@ -440,8 +444,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(Fp4GemmArgs p
           tc::tmem_ld32(base + u * 64, x0);
           tc::tmem_ld32(base + u * 64 + 32, x1);
           if (PAIR ? part == 0 && i == 0 : true) release();
-          if (n0 + u * 64 < p.N) store32(p, row, n0 + u * 64, rs, x0);
-          if (n0 + u * 64 + 32 < p.N) store32(p, row, n0 + u * 64 + 32, rs, x1);
+          if (n0 + u * 64 < p.N) store32(p, row, n0 + u * 64, split_scale(rs), x0);
+          if (n0 + u * 64 + 32 < p.N) store32(p, row, n0 + u * 64 + 32, split_scale(rs), x1);
         }
       }
     }

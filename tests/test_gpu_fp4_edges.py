@@ -5,7 +5,7 @@ import torch
 
 from glm53.ops import fp4
 from glm53.ops import kernels as K
-from test_gpu_fp4 import F32, FMTS, act_tol, acts, gated, h_slack, quant, sums_tol, weight
+from test_gpu_fp4 import BF, F32, FMTS, act_tol, acts, gated, h_slack, quant, sums_tol, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,56 @@ def test_linear_repeats_itself_over_many_row_blocks(m, n, k):
     tol = sums_tol(x.double(), wq) + act_tol(x.double(), wq, fmt)
     assert ((y[:, some].double() - x.double() @ wq.t()).abs() <= tol).all()
     fp4.check_errors()
+
+
+PATHS = [(150, 200, True), (2600, 1800, True)]
+
+
+def far(m, n, k=256):
+    x, w = acts(m, k, m), weight(n, k, 5)
+    x[0] = 2.0 ** -64
+    x[1] = 2.0 ** 80
+    x[1, ::2] *= -1
+    x[2] = 2.0 ** 118
+    w[0] = 2.0 ** -65
+    w[1] = 2.0 ** 80
+    w[2] = 2.0 ** -4
+    w[3] *= 2.0 ** -60
+    return x, w
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n,act4", PATHS)
+def test_linear_scales_far_apart(fmt, m, n, act4):
+    """Results inside fp32's range come out whatever the scales of the two rows are."""
+    x, w = far(m, n)
+    w4, wq = fp4.quantize4(w, fmt), quant(w, fmt)
+    a = quant(x, fmt) if act4 else x.double()
+    y = fp4.linear4(x, w4, torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32, act4=act4).double()
+    mag = a.abs() @ wq.abs().t()
+    # where the sum of magnitudes nears fp32's largest a partial sum may be an infinity; a last rounding below 2^-126 is off by
+    # at most 2^-149
+    tol = sums_tol(a, wq) + (0 if act4 else act_tol(a, wq, fmt)) + 2.0 ** -149
+    fine = mag < 2.0 ** 127
+    assert fine[0].all() and fine[2, 0] and fine[2, 2] and fine[2, 4:].all()
+    assert ((y - a @ wq.t()).abs() <= tol)[fine].all()
+
+
+@pytest.mark.parametrize("m,n,act4", PATHS)
+def test_linear_zero_sums_of_large_rows(m, n, act4):
+    """nvfp4: codes and block scales of +-2^80 and 2^80 sum to 0 exactly, and 0 times any row scales is 0."""
+    x, w = far(m, n)
+    y = fp4.linear4(x, fp4.quantize4(w, "nvfp4"), torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32, act4=act4)
+    assert y[1, 0] == 0 and y[1, 1] == 0 and y[1, 2] == 0
+
+
+@pytest.mark.parametrize("m,width", [(150, 160), (2600, 928)])
+def test_mlp_zero_gates_of_large_rows(m, width):
+    """A gate whose sum is 0 gives 0, with 4-bit activations, too, whatever its row scales."""
+    k = 256
+    x = acts(m, k, m)
+    x[1::2] = 2.0 ** 80
+    x[1::2, ::2] *= -1
+    mlp = fp4.pack_mlp4(torch.full((width, k), 2.0 ** 80, dtype=BF, device="cuda"), weight(width, k, 2), weight(64, width, 3))
+    y = fp4.mlp4(x, mlp, torch.empty(m, 64, dtype=F32, device="cuda"), 10.0, act4=True)
+    assert (y[1::2] == 0).all() and torch.isfinite(y).all()
