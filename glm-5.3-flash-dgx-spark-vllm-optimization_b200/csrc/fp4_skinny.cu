@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
     const bool swi = p.mode == GEMV_SWIGLU;
     const bool direct = CL == 1 && !swi;              // rows finished where they are read
     // this thread's first share of the finishing: four tokens of one row (of a pair of rows)
-    const int f_q = et / rows, f_row = et - f_q * rows, f_half = swi ? 0 : f_q & 1;
+    const int f_q = et / rows, f_row = et - f_q * rows;
     pdl_wait();
     if constexpr (INLINE) {
       // a thread per 8 elements of the slice (the plan sees to it that there are no more than threads)
@@ -432,11 +432,8 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
       const int M = min(p.M - x0, pl.group);
       const uint32_t rbar = tc::saddr(&recv_bar[blk & 1]);
       if (CL > 1 && et == 0) bulk_expect(&recv_bar[blk & 1], (uint32_t)((CL - 1) * 2 * rows * ((M + 3) & ~3) * 4));
-      // scales of the rows that this thread finishes (first): loaded under the main loop
-      float rs = 1.f, ru = 1.f;
-      const int n_own = nb * 128 + (direct ? r : j_lo + f_row + f_half * 64);
-      if (NV && n_own < p.N) rs = __ldcg(p.row_scale + n_own);
-      if (NV && swi && n_own + 64 < p.N) ru = __ldcg(p.row_scale + n_own + 64);
+      // scale of this thread's weight row: loaded under the main loop
+      const RowScale ws = split_scale(NV && nb * 128 + r < p.N ? __ldcg(p.row_scale + nb * 128 + r) : 1.f);
       // factors of the rows of x: lane l those of l, l + 32, ..
       constexpr int kXf = T == 1 ? 4 : 1;
       float xf[kXf];
@@ -476,12 +473,12 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
             for (int t = T - 1; t >= 0; --t)           // small terms first
               sum[i] = NV ? fmaf(v[(j4 + i) * T + t], 1.f / (float)(1 << (3 * t)), sum[i]) : sum[i] + v[(j4 + i) * T + t];
             // rows past M: never used
-            if (NV) sum[i] *= __shfl_sync(0xffffffffu, f, (m0 + i) & 31);
+            if (NV) sum[i] = sum[i] * (__shfl_sync(0xffffffffu, f, (m0 + i) & 31) * ws.a) * ws.b;
           }
           if (direct) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (m0 + i < M && nb * 128 + r < p.N) store1(p, x0 + m0 + i, nb * 128 + r, sum[i] * rs);
+              if (m0 + i < M && nb * 128 + r < p.N) store1(p, x0 + m0 + i, nb * 128 + r, sum[i]);
           } else if (owner == rank) {
             *reinterpret_cast<float4*>(dst + m0) = make_float4(sum[0], sum[1], sum[2], sum[3]);
           } else {
@@ -515,16 +512,15 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
           }
         }
         const int n = nb * 128 + j_lo + row + hf * 64;
-        float vs[4] = {v.x, v.y, v.z, v.w};
+        const float vs[4] = {v.x, v.y, v.z, v.w};
         const float us[4] = {w.x, w.y, w.z, w.w};
         if (swi) {
           const int col = nb * 64 + j_lo + row;
           if (col >= p.width) continue;
-          const float sg = !NV || own ? rs : __ldcg(p.row_scale + n), su = !NV || own ? ru : __ldcg(p.row_scale + n + 64);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (tok + i >= M) break;
-            float g = vs[i] * sg, h = us[i] * su;
+            float g = vs[i], h = us[i];
             // written so that a NaN stays one
             g = g > p.limit ? p.limit : g;
             h = h > p.limit ? p.limit : h < -p.limit ? -p.limit : h;
@@ -532,10 +528,9 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
           }
         } else {
           if (n >= p.N) continue;
-          const float sc = !NV || own ? rs : __ldcg(p.row_scale + n);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (tok + i < M) store1(p, x0 + tok + i, n, vs[i] * sc);
+            if (tok + i < M) store1(p, x0 + tok + i, n, vs[i]);
         }
       }
       if (CL > 1 && u + pl.clusters < pl.units) sk_sync();   // this block is read: its sums of the next may go out
