@@ -64,8 +64,9 @@ __device__ __forceinline__ uint32_t dup_bf16(float v) {
 // 8 codes -> 8 bf16, times s.  The bits of a code (sign, two of exponent, one of mantissa) at 15 and 8..6 of a bf16 are the
 // value x 2^-126, its subnormal 1/2 included: a byte permutation lays two codes into the halves of a word (its sign mode
 // gives the zero bytes), one multiplication copies them to both places, a mask keeps the bits wanted.  The scale brings the
-// exponent: for nvfp4 s = scale x 2^118, so the result is 2^-8 of the weight (the epilogue makes it up); an E8M0 scale may be
-// as large as a bf16, so mxfp4 multiplies twice.  Every product is exact.
+// exponent: for nvfp4 s = scale x 2^110, so the result is 2^-16 of the weight over its row's scale, at most 0.041 (the epilogue
+// makes it up): sums do not overflow that the row's scale brings back; an E8M0 scale may be as large as a bf16, so mxfp4
+// multiplies twice.  Every product is exact.
 template <bool NV>
 __device__ __forceinline__ uint4 widen8(uint32_t w, uint32_t s) {
   const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;            // codes 0, 2, 4, 6 and 1, 3, 5, 7
@@ -300,8 +301,8 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
         if constexpr (NV) {
           const uint32_t h = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(sp));
           const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-          s0 = dup_bf16(f.x * 0x1p118f);
-          s1 = dup_bf16(f.y * 0x1p118f);
+          s0 = dup_bf16(f.x * 0x1p110f);
+          s1 = dup_bf16(f.y * 0x1p110f);
         } else {
           s0 = s1 = dup_bf16(e8m0_to_f32(*sp));
         }
@@ -334,15 +335,16 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
     const int ce = min(M, cb + kPass);
     if (warp >= kRoles) {
       const int ww = warp - kRoles, r = (warp & 3) * 32 + lane, n = nb * 128 + r;
+      // the row's scale and the 2^16 of the widening, in an order that neither overflows (2^117 * 2^16) nor underflows
       const float rs = NV && n < p.N ? __ldcg(p.row_scale + n) : 1.f;
+      const float f0 = rs > 1.f ? rs : rs * 0x1p16f, f1 = rs > 1.f ? 0x1p16f : 1.f;
       for (int c0 = cb + (ww >> 2) * 32; c0 < ce; c0 += kWiden / 4 * 32) {
         float v[32];
         if (live) tc::tmem_ld32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           if (c0 + i >= ce) break;
-          if (NV) v[i] *= 256.f;
-          part[(c0 + i - cb) * kPartLd + r] = v[i] * rs;
+          part[(c0 + i - cb) * kPartLd + r] = NV ? v[i] * f0 * f1 : v[i];
         }
       }
     }

@@ -71,8 +71,8 @@ def test_linear_repeats_itself_over_many_row_blocks(m, n, k):
     fp4.check_errors()
 
 
-PATHS = [(3, 200, False), (12, 200, False), (40, 200, False), (90, 200, False), (20, 200, True), (128, 200, True),
-         (150, 200, True), (2600, 1800, True)]
+PATHS = [(3, 200, False), (12, 200, False), (40, 200, False), (90, 200, False), (150, 200, False), (700, 200, False),
+         (20, 200, True), (128, 200, True), (150, 200, True), (2600, 1800, True)]
 
 
 def far(m, n, k=256):
