@@ -559,9 +559,4 @@ cudaError_t g53_fp4_exact(const Fp4ExactArgs& p, cudaStream_t st) {
   return p.nv ? fp4::launch_exact<true>(q, st) : fp4::launch_exact<false>(q, st);
 }
 
-cudaError_t g53_fp4_exact_error(int* code) {
-  const int z = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(code, fp4::g_exact_err, sizeof(int));
-  if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(fp4::g_exact_err, &z, sizeof(int));
-  return e;
-}
+cudaError_t g53_fp4_exact_error(int* code, cudaStream_t st) { return fp4::copy_error(fp4::g_exact_err, code, st); }

@@ -536,9 +536,4 @@ cudaError_t g53_fp4_gemm(const Fp4GemmArgs& p, cudaStream_t st) {
   return p.nv ? fp4::gemm_t<true>(q, dev, sms, st) : fp4::gemm_t<false>(q, dev, sms, st);
 }
 
-cudaError_t g53_fp4_gemm_error(int* code) {
-  const int z = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(code, fp4::g_gemm_err, sizeof(int));
-  if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(fp4::g_gemm_err, &z, sizeof(int));
-  return e;
-}
+cudaError_t g53_fp4_gemm_error(int* code, cudaStream_t st) { return fp4::copy_error(fp4::g_gemm_err, code, st); }

@@ -724,9 +724,4 @@ cudaError_t g53_fp4_skinny(const Fp4SkinnyArgs& p, cudaStream_t st) {
   return p.nv ? fp4::skinny_t<true>(p, st) : fp4::skinny_t<false>(p, st);
 }
 
-cudaError_t g53_fp4_skinny_error(int* code) {
-  const int z = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(code, fp4::g_skinny_err, sizeof(int));
-  if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(fp4::g_skinny_err, &z, sizeof(int));
-  return e;
-}
+cudaError_t g53_fp4_skinny_error(int* code, cudaStream_t st) { return fp4::copy_error(fp4::g_skinny_err, code, st); }

@@ -117,5 +117,12 @@ __device__ __forceinline__ void bulk_expect(uint64_t* b, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::saddr(b)), "r"(bytes) : "memory");
 }
 
+// an error word of the current device to *code behind the work on `st`, or (null) cleared
+inline cudaError_t copy_error(const int& word, int* code, cudaStream_t st) {
+  if (code) return cudaMemcpyFromSymbolAsync(code, word, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  static const int z = 0;
+  return cudaMemcpyToSymbolAsync(word, &z, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+}
+
 }  // namespace fp4
 }  // namespace g53

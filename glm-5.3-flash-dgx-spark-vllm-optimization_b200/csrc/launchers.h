@@ -470,7 +470,8 @@ struct Fp4GemmArgs {
   int vec;                             // set by the launcher: 16-byte epilogue stores allowed
 };
 cudaError_t g53_fp4_gemm(const Fp4GemmArgs& p, cudaStream_t st);
-// first error code recorded on the current device by a bounded wait of these kernels (0: none); clears it
-cudaError_t g53_fp4_skinny_error(int* code);
-cudaError_t g53_fp4_exact_error(int* code);
-cudaError_t g53_fp4_gemm_error(int* code);
+// last error code recorded on the current device by a bounded wait of these kernels (0: none), copied to *code behind the
+// work on the stream; code null: cleared
+cudaError_t g53_fp4_skinny_error(int* code, cudaStream_t st);
+cudaError_t g53_fp4_exact_error(int* code, cudaStream_t st);
+cudaError_t g53_fp4_gemm_error(int* code, cudaStream_t st);

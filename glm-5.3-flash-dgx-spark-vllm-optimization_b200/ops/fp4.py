@@ -151,9 +151,12 @@ def mlp4(x: torch.Tensor, m: MLP4, y: torch.Tensor, limit: float, mode: int = GE
     return y
 
 
-def check_errors(device=None) -> None:
-    """Raise if a bounded wait of these kernels ran out on ``device`` since the last check (synchronises)."""
+def check_errors(device=None, wait: bool = True) -> None:
+    """Raise if a bounded wait of these kernels ran out on ``device`` since the last check; what they wrote then is not to be
+    used.  Waits for every stream of the device, or (``wait=False``) for the current one only.  Not inside a capture."""
     dev = torch.device("cuda" if device is None else device)
+    if wait:
+        torch.cuda.synchronize(dev)
     code = _ext.require().fp4_error(torch.cuda.current_device() if dev.index is None else dev.index)
     if code:
         raise RuntimeError(f"4-bit kernels: a bounded wait ran out (code {code:#x})")

@@ -123,3 +123,12 @@ def test_mlp_zero_gates_of_large_rows(m, width):
     mlp = fp4.pack_mlp4(torch.full((width, k), 2.0 ** 80, dtype=BF, device="cuda"), weight(width, k, 2), weight(64, width, 3))
     y = fp4.mlp4(x, mlp, torch.empty(m, 64, dtype=F32, device="cuda"), 10.0, act4=True)
     assert (y[1::2] == 0).all() and torch.isfinite(y).all()
+
+
+def test_check_errors_waits_for_every_stream():
+    s, ev = torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(100_000_000)                  # about 50 ms
+        ev.record()
+    fp4.check_errors()
+    assert ev.query()
