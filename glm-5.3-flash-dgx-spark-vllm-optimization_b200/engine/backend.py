@@ -10,6 +10,7 @@ import torch
 
 from ..models.drafter import BlockDrafter
 from ..models.runtime import Graphed, Runtime, RuntimeConfig
+from ..ops import fp4
 from ..ops import kernels as K
 from ..ops.sampling import GreedySampler
 
@@ -40,6 +41,7 @@ class GPUBackend:
         self.cuda_graphs = cuda_graphs
         self._graphs: dict = {}
         self.vocab = self.cfg.vocab
+        self.mlp4 = any((lw.mlp or lw.moe.shared).four is not None for lw in weights.layers)
         # KDA state checkpoints (prefix cache): copies of every KDA layer's state and conv window
         self.ck_S = [torch.zeros((checkpoints,) + S.shape[1:], dtype=S.dtype, device=dev) for S in
                      getattr(self.rt, "S_pool", [])] if checkpoints else []
@@ -111,6 +113,8 @@ class GPUBackend:
         out = self.sampler(logits).tolist()          # synchronises: kernel error words can be read now
         if self.rt.px is not None:
             self.rt.px.check()
+        if self.mlp4:
+            fp4.check_errors(logits.device, wait=False)
         return out
 
     @torch.no_grad()

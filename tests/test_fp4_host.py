@@ -1,0 +1,30 @@
+"""Host side of the 4-bit MLPs in the engine (no GPU needed)."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from glm53.engine.backend import GPUBackend
+from glm53.ops import _ext
+
+
+def backend(mlp4):
+    b = GPUBackend.__new__(GPUBackend)
+    b.sampler, b.rt, b.mlp4 = (lambda lg: lg.argmax(-1)), SimpleNamespace(px=None), mlp4
+    return b
+
+
+def test_argmax_raises_when_a_wait_of_the_4bit_kernels_ran_out(monkeypatch):
+    words = [0, 0x6b40]
+    asked = []
+    monkeypatch.setattr(_ext, "require", lambda: SimpleNamespace(fp4_error=lambda d: asked.append(d) or words.pop(0)))
+    logits = SimpleNamespace(device=torch.device("cuda", 3), argmax=lambda dim: torch.tensor([5]))
+    assert backend(True).argmax(logits) == [5]
+    with pytest.raises(RuntimeError, match="bounded wait ran out .code 0x6b40"):
+        backend(True).argmax(logits)
+    assert asked == [3, 3]
+
+
+def test_argmax_does_not_ask_without_4bit_mlps(monkeypatch):
+    monkeypatch.setattr(_ext, "require", lambda: pytest.fail("asked"))
+    assert backend(False).argmax(torch.eye(3)) == [0, 1, 2]
