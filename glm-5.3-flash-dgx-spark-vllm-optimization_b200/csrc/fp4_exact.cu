@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
     __syncwarp();
   } else if (warp == 1) {
     if (elect_one()) {
+      pdl_wait();                                     // bounded waits must not run while an earlier kernel does
       bool ok = true;
       int s = 0, ph = 0;
       if (side == 1) {
@@ -283,6 +284,7 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
     }
     __syncwarp();
   } else {
+    pdl_wait();
     const int ww = warp - kRoles, set = ww >> 3;
     const int row = (ww & 7) * 16 + (lane >> 1), half = lane & 1;            // 32 of the stage's 64 columns of a row
     const int flip = (row & 7) << 4;                    // the swizzle of this row
@@ -325,7 +327,6 @@ __global__ void __launch_bounds__(kExThreads, 1) fp4_exact_kernel(const __grid_c
         if (live && st + kSets < n_st) live = look(&wfull[w], wph, fail, 4);
       }
     }
-    pdl_wait();
     if (live) live = tc::warp_wait(&tfull, 0, fail, &g_exact_err, 6);
     tc::fence_after();
   }

@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(kSkThreads, WIDE ? 1 : 2) fp4_skinny_kernel(Fp
     if (CL > 1) cluster_wait();
   } else if (warp == 1) {
     if (elect_one()) {
+      pdl_wait();                                     // its bounded waits must not run while an earlier kernel does
       const int ksteps = (p.K + 63) / 64;
       uint32_t it = 0, blk = 0;
       bool ok = true;
