@@ -91,11 +91,12 @@ __device__ __forceinline__ uint32_t block_amax(uint32_t am) {
   am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
   return NV ? am : max(am, __shfl_xor_sync(0xffffffffu, am, 2));
 }
+// (from L2, like everything that an earlier programmatic launch may have written)
 __device__ __forceinline__ uint4 load8(const uint16_t* x, bool vec) {
-  if (vec) return *reinterpret_cast<const uint4*>(x);
+  if (vec) return __ldcg(reinterpret_cast<const uint4*>(x));
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)x[2 * i] | ((uint32_t)x[2 * i + 1] << 16);
+  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldcg(x + 2 * i) | ((uint32_t)__ldcg(x + 2 * i + 1) << 16);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ int exponent(uint32_t bits) { return (int)(bits >> 23) - 127; }

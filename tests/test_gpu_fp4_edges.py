@@ -132,3 +132,26 @@ def test_check_errors_waits_for_every_stream():
         ev.record()
     fp4.check_errors()
     assert ev.query()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,act4", [(1, False), (8, False), (12, False), (30, False), (90, False), (90, True), (150, False),
+                                    (150, True)])
+def test_products_chained_through_one_pair_of_buffers(fmt, m, act4):
+    """Each product reads what the launch before it wrote, and writes what that one read: the bits of a run with a wait after
+    every call."""
+    k = 1024
+    w4 = fp4.quantize4(weight(k, k, 4), fmt)
+    x = acts(m, k, 1)
+
+    def chain(wait):
+        bufs = [x.clone(), torch.empty_like(x)]
+        for i in range(40):
+            fp4.linear4(bufs[i % 2], w4, bufs[1 - i % 2], act4=act4)
+            if wait:
+                torch.cuda.synchronize()
+        return bufs[0]
+    want = chain(True)
+    assert torch.isfinite(want).all() and want.any()
+    assert all(torch.equal(chain(False), want) for _ in range(5))
+    fp4.check_errors()
