@@ -41,9 +41,9 @@ class LLMOptions:
     block_verify: bool = False          # sampled requests: block verification instead of standard
     mixed_prefill_chunk: int = 0        # prefill tokens per step while requests decode (0: the whole chunk)
     ep: bool = False                    # routed experts expert-parallel over the ranks (parallel/ep.py)
+    sp_mla: bool = os.environ.get("GLM53_SP_MLA", "1") == "1"   # row-parallel MLA in sequence-parallel prefill
     mlp4: str | None = None             # dense MLPs and shared experts in 4 bits: "nvfp4" or "mxfp4" (one GPU)
     mlp4_act4: bool = False             # with mlp4: 4-bit activations, too, in prefill chunks
-    sp_mla: bool = os.environ.get("GLM53_SP_MLA", "1") == "1"   # row-parallel MLA in sequence-parallel prefill
 
 
 class LLM:

@@ -28,3 +28,12 @@ def test_argmax_raises_when_a_wait_of_the_4bit_kernels_ran_out(monkeypatch):
 def test_argmax_does_not_ask_without_4bit_mlps(monkeypatch):
     monkeypatch.setattr(_ext, "require", lambda: pytest.fail("asked"))
     assert backend(False).argmax(torch.eye(3)) == [0, 1, 2]
+
+
+def test_option_order_of_positional_callers():
+    """The 4-bit options stand behind the ones that were there: sp_mla keeps its place."""
+    import dataclasses
+
+    from glm53.api.offline import LLMOptions
+    names = [f.name for f in dataclasses.fields(LLMOptions)]
+    assert names[names.index("ep") + 1] == "sp_mla" and names[-2:] == ["mlp4", "mlp4_act4"]
