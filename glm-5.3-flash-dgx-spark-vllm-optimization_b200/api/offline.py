@@ -43,7 +43,11 @@ class LLMOptions:
     ep: bool = False                    # routed experts expert-parallel over the ranks (parallel/ep.py)
     sp_mla: bool = os.environ.get("GLM53_SP_MLA", "1") == "1"   # row-parallel MLA in sequence-parallel prefill
     mlp4: str | None = None             # dense MLPs and shared experts in 4 bits: "nvfp4" or "mxfp4" (one GPU)
-    mlp4_act4: bool = False             # with mlp4: 4-bit activations, too, in prefill chunks
+    mlp4_act4: bool = False             # with mlp4: 4-bit activations, too, in forwards of more rows than a decode window's
+
+    def __post_init__(self):
+        if self.mlp4_act4 and self.mlp4 is None:
+            raise ValueError("mlp4_act4 (4-bit activations) needs mlp4: there is no 4-bit MLP without it")
 
 
 class LLM:

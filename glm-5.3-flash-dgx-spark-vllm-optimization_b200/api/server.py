@@ -514,7 +514,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--no-cuda-graphs", action="store_true")
     ap.add_argument("--mlp4", choices=["nvfp4", "mxfp4"], default=None,
                     help="dense MLPs and shared experts in 4 bits (one GPU)")
-    ap.add_argument("--mlp4-act4", action="store_true", help="with --mlp4: 4-bit activations in prefill chunks, too")
+    ap.add_argument("--mlp4-act4", action="store_true", help="with --mlp4: 4-bit activations, too, beyond a decode window's rows")
     ap.add_argument("--served-model-name", default="glm-5.3-flash")
     ap.add_argument("--api-key", default=None, help="require Authorization: Bearer <key> on /v1 routes")
     ap.add_argument("--no-reasoning-parser", action="store_true")

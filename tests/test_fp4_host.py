@@ -37,3 +37,13 @@ def test_option_order_of_positional_callers():
     from glm53.api.offline import LLMOptions
     names = [f.name for f in dataclasses.fields(LLMOptions)]
     assert names[names.index("ep") + 1] == "sp_mla" and names[-2:] == ["mlp4", "mlp4_act4"]
+
+
+def test_act4_alone_is_refused():
+    from glm53.api.offline import LLMOptions
+    from glm53.api.server import build_parser, options_from_args
+    with pytest.raises(ValueError, match="mlp4_act4 .* needs mlp4"):
+        LLMOptions(mlp4_act4=True)
+    with pytest.raises(ValueError, match="mlp4_act4 .* needs mlp4"):
+        options_from_args(build_parser().parse_args(["--mlp4-act4"]))
+    assert LLMOptions(mlp4="mxfp4", mlp4_act4=True).mlp4_act4
