@@ -184,54 +184,57 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(Fp4DequantArgs p) {
   if (row >= p.R) return;
   const int rr = (int)(row % kTileRows);
   const float rs = NV ? __ldcg(p.row_scale + row) : 1.f;
-  const int kt1 = min(KT, ((int)blockIdx.y + 1) * kDqTiles);
-#pragma unroll 4
-  for (int kt = blockIdx.y * kDqTiles; kt < kt1; ++kt) {
-    const int64_t tile = (row / kTileRows) * KT + kt;
-    const int64_t k0 = (int64_t)kt * kTileK + lane * 8;
-    if (k0 >= p.K) continue;
-    const uint32_t w =
-        __ldcg(reinterpret_cast<const uint32_t*>(p.codes + tile * kTileBytes + chunk_off(rr, lane >> 2) + (lane & 3) * 4));
-    const uint32_t sb = __ldcg(p.scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, NV ? lane >> 1 : lane >> 2));
-    const float s = NV ? e4m3_to_f32(sb) * rs : e8m0_to_f32(sb);
-    uint32_t h[4];
-    e2m1x8_to_f16(w, h);
-    float v[8];
+  // (a grid has 65535 CTAs in y: longer rows go round)
+  for (int kt0 = blockIdx.y * kDqTiles; kt0 < KT; kt0 += gridDim.y * kDqTiles) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-      v[2 * i] = f.x * s;
-      v[2 * i + 1] = f.y * s;
-    }
-    const int64_t off = row * p.ldy + k0;
-    if constexpr (OUT == 2) {
-      float* y = reinterpret_cast<float*>(p.y) + off;
-      if (p.vec) {
-        reinterpret_cast<float4*>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = v[i];
-      }
-    } else {
-      uint32_t o[4];
+    for (int q = 0; q < kDqTiles; ++q) {
+      const int kt = kt0 + q;
+      const int64_t tile = (row / kTileRows) * KT + kt;
+      const int64_t k0 = (int64_t)kt * kTileK + lane * 8;
+      if (k0 >= p.K) continue;
+      const uint32_t w =
+          __ldcg(reinterpret_cast<const uint32_t*>(p.codes + tile * kTileBytes + chunk_off(rr, lane >> 2) + (lane & 3) * 4));
+      const uint32_t sb = __ldcg(p.scales + tile * Fmt<NV>::kScaleBytes + scale_off(rr, NV ? lane >> 1 : lane >> 2));
+      const float s = NV ? e4m3_to_f32(sb) * rs : e8m0_to_f32(sb);
+      uint32_t h[4];
+      e2m1x8_to_f16(w, h);
+      float v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (OUT == 0) {
-          __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-          o[i] = *reinterpret_cast<uint32_t*>(&b);
-        } else {
-          o[i] = f32x2_to_f16x2(v[2 * i], v[2 * i + 1]);
-        }
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        v[2 * i] = f.x * s;
+        v[2 * i + 1] = f.y * s;
       }
-      uint16_t* y = reinterpret_cast<uint16_t*>(p.y) + off;
-      if (p.vec) {
-        *reinterpret_cast<uint4*>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+      const int64_t off = row * p.ldy + k0;
+      if constexpr (OUT == 2) {
+        float* y = reinterpret_cast<float*>(p.y) + off;
+        if (p.vec) {
+          reinterpret_cast<float4*>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = v[i];
+        }
       } else {
+        uint32_t o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          y[2 * i] = (uint16_t)(o[i] & 0xffffu);
-          y[2 * i + 1] = (uint16_t)(o[i] >> 16);
+          if constexpr (OUT == 0) {
+            __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            o[i] = *reinterpret_cast<uint32_t*>(&b);
+          } else {
+            o[i] = f32x2_to_f16x2(v[2 * i], v[2 * i + 1]);
+          }
+        }
+        uint16_t* y = reinterpret_cast<uint16_t*>(p.y) + off;
+        if (p.vec) {
+          *reinterpret_cast<uint4*>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[2 * i] = (uint16_t)(o[i] & 0xffffu);
+            y[2 * i + 1] = (uint16_t)(o[i] >> 16);
+          }
         }
       }
     }
@@ -257,7 +260,7 @@ static cudaError_t quantize_t(const Fp4QuantArgs& p, cudaStream_t st) {
 
 template <bool NV>
 static cudaError_t dequant_t(const Fp4DequantArgs& p, cudaStream_t st) {
-  const dim3 grid((unsigned)((p.R + 7) / 8), (tiles_k(p.K) + kDqTiles - 1) / kDqTiles);
+  const dim3 grid((unsigned)((p.R + 7) / 8), std::min(65535, (tiles_k(p.K) + kDqTiles - 1) / kDqTiles));
   switch (p.out) {
     case 0: return g53_launch_pdl(fp4_dequant_kernel<NV, 0>, grid, dim3(256), 0, st, 1, p);
     case 1: return g53_launch_pdl(fp4_dequant_kernel<NV, 1>, grid, dim3(256), 0, st, 1, p);

@@ -155,3 +155,14 @@ def test_products_chained_through_one_pair_of_buffers(fmt, m, act4):
     assert torch.isfinite(want).all() and want.any()
     assert all(torch.equal(chain(False), want) for _ in range(5))
     fp4.check_errors()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_longest_rows(fmt):
+    """A row of more than 65535 times 1024 columns, there and back."""
+    k = 65535 * 1024 + 4096 + 32
+    x = acts(1, k, 1)
+    y = fp4.dequantize4(fp4.quantize4(x, fmt))
+    torch.cuda.synchronize()
+    ref = quant(x, fmt)
+    assert torch.equal(y.double(), ref)
