@@ -1,11 +1,12 @@
 // 4-bit floating-point matrices (e2m1 codes with block scales): storage layout and element helpers shared by the
-// quantiser (fp4_quant.cu), the small-M product (fp4_gemv.cu) and the tcgen05 product (fp4_gemm.cu).
+// quantiser (fp4_quant.cu), the small-M product (fp4_skinny.cu), the product that widens the weights (fp4_exact.cu) and the
+// product of two 4-bit matrices (fp4_gemm.cu).
 //
 // Value of an element: e2m1(code) * block scale * row scale.
 //   mxfp4   blocks of 32 along K, block scale 2^(b - 127) (one byte b, E8M0; 255 = NaN), no row scale
 //   nvfp4   blocks of 16 along K, block scale e4m3 (0x7F = NaN), fp32 row scale (a power of two)
 //
-// Storage: a matrix [R, K] is kept as shared-memory images, so both products fetch a 128 x 256 tile with one
+// Storage: a matrix [R, K] is kept as shared-memory images, so every product fetches a 128 x 256 tile with one
 // contiguous cp.async.bulk per array (no tensor map, full DRAM bursts, any K that is a multiple of the block):
 //   codes   [ceil(R / 128)][ceil(K / 256)][128 rows][128 bytes]: a row's 256 codes (low nibble first) in the 128-byte
 //           swizzle of the K-major tcgen05 operand: 16-byte chunk c (32 codes) of row r sits at chunk c ^ (r % 8)

@@ -7,10 +7,11 @@ times (nvfp4) its row's scale:
 * ``"nvfp4"``: blocks of 16 along K with an e4m3 scale, and a power of two per row (the smallest 2^k with the row's
   largest magnitude <= 448 * 6 * 2^k, at least 2^-100); 4.5 bits per element.
 * ``"mxfp4"``: blocks of 32 along K with a power-of-two scale (the smallest 2^e with the block's largest magnitude <=
-  6 * 2^e, so nothing saturates); 4.25 bits per element.
+  6 * 2^e, at least 2^-126, so nothing saturates); 4.25 bits per element.
 
-Codes are rounded to nearest, ties to even.  Values are exact in bf16, so reading back loses nothing more.  An infinity
-or NaN makes its block (mxfp4) or row (nvfp4) read back as NaN.
+Codes are rounded to nearest, ties to even.  Values are exact in bf16, so reading back loses nothing more (a magnitude
+within a code's rounding of bf16's largest can round up past it, and reads back as infinity).  An infinity or NaN makes its
+block (mxfp4) or row (nvfp4) read back as NaN.
 
 A matrix is stored as the shared-memory images the kernels load (csrc/fp4.cuh), rows in blocks of 128 and columns in tiles
 of 256.  The operators launch on the current stream of the tensors' device and can be captured in a CUDA graph; weights
@@ -20,12 +21,13 @@ Row counts and numerics of ``linear4`` / ``mlp4``:
 
 * ``act4=False``, and up to 16 rows always: bf16 activations (W4A16).  Up to 96 rows each is expanded into 4-bit terms
   for the 4-bit tensor cores, which leaves out at most 2^-22 of the largest magnitude of its block of 16 (nvfp4) or 32
-  (mxfp4) columns, in nvfp4 2^-39 of the row's where that is more; with more rows the weights are widened to bf16 inside
-  the product, exactly.  A row's result thus does not depend on the other rows, but its last bits on their number;
+  (mxfp4) columns, in nvfp4 2^-39 of the row's where that is more, and up to 2^-124 of rows below 2^-85 (nvfp4) or blocks
+  below 2^-105 (mxfp4); with more rows the weights are widened to bf16 inside the product, exactly.  A row's result thus
+  does not depend on the other rows, but its last bits on their number;
 * ``act4=True``, more than 16 rows: activations are quantised per row to the weights' format and multiplied on the
   block-scaled tensor cores (W4A4).
 
-Sums are fp32 and added in a fixed order.
+Sums are fp32 and added in a fixed order: a call repeats itself bit for bit.
 """
 
 from __future__ import annotations

@@ -166,3 +166,37 @@ def test_longest_rows(fmt):
     torch.cuda.synchronize()
     ref = quant(x, fmt)
     assert torch.equal(y.double(), ref)
+
+
+def tiny(rows, k):
+    """Rows around 2^-70, 2^-95, 2^-105, 2^-120 and among bf16's subnormals."""
+    x = acts(rows, k, 3)
+    for i, e in enumerate((-70, -95, -105, -120, -128)):
+        x[i] = (x[i].double() * 2.0 ** e).to(BF)
+    return x
+
+
+def test_quantize_smallest_magnitudes():
+    x = tiny(6, 256)
+    assert torch.equal(fp4.dequantize4(fp4.quantize4(x, "nvfp4"), F32).double(), quant(x, "nvfp4"))
+    # mxfp4: scales from 2^-126; from there on codes are multiples of 2^-127
+    b = x.double().view(6, -1, 32)
+    s = torch.exp2(torch.ceil(torch.log2(b.abs().amax(-1, keepdim=True) / 6))).clamp_min(2.0 ** -126)
+    low = s == 2.0 ** -126
+    assert low[4].all() and not low[0].any()
+    y = fp4.dequantize4(fp4.quantize4(x, "mxfp4"), F32).double().view(b.shape)
+    q = b.abs() / s
+    # half the distance of the two codes around q: 1/4 below 2, 1/2 below 4, 1 below 6
+    assert ((y - b).abs() <= s * torch.where(q <= 2, 0.25, torch.where(q <= 4, 0.5, 1.0))).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m", [6, 12, 40, 150])
+def test_linear_smallest_magnitudes(fmt, m):
+    n, k = 136, 512
+    x, w = tiny(m, k), weight(n, k, 5)
+    w4, wq = fp4.quantize4(w, fmt), quant(w, fmt)
+    y = fp4.linear4(x, w4, torch.empty(m, n, dtype=F32, device="cuda"), K.GEMV_F32)
+    # what the expansion (and, widened, fp32's own range) leaves out of an element of such rows: 2^-124
+    tol = sums_tol(x.double(), wq) + act_tol(x.double(), wq, fmt) + 2.0 ** -124 * wq.abs().sum(1)
+    assert ((y.double() - x.double() @ wq.t()).abs() <= tol).all()
