@@ -148,7 +148,7 @@ def mlp4(x: torch.Tensor, m: MLP4, y: torch.Tensor, limit: float, mode: int = GE
     h is held in bf16, or with ``act4`` (above 16 rows) in the weights' 4-bit format; nvfp4 then takes its row scale from
     max(limit, 0.2785) * limit (limit must be finite), which no |h| exceeds, instead of the row's maximum, so that h is
     quantised where it is computed.  A block of h then keeps its precision down to about 2^-14 of that bound and is 0 from
-    about 2^-18 of it on."""
+    about 2^-18 of it on; nvfp4 gate and up rows with magnitudes above 2^100 may then overflow on the way."""
     _ext.require().fp4_mlp(x, m.gu.handle, m.down.handle, y, limit, mode, act4)
     return y
 
